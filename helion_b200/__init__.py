@@ -8,6 +8,7 @@ library ``libhelion_b200.so`` declared in ``include/helion_b200.h``.
 """
 
 from . import layouts
+from .fused_linear import linear
 from .grouped import grouped_gemm
 from .grouped import grouped_gemm_deepgemm
 from .grouped import grouped_gemm_direct
@@ -48,6 +49,7 @@ __all__ = [
     "moe_matmul_ogs",
     "moe_matmul_ogs_helion_kernel_args_gen",
     "layouts",
+    "linear",
     "nvfp4_gemv_bf16in",
     "nvfp4_gemv_bf16in_batched",
     "nvfp4_gemv_fp4in",

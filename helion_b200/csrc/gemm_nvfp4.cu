@@ -623,7 +623,9 @@ int peer_device_status(int reset);
 int gemv_tc_device_status(int reset);
 int fp8_device_status(int reset);
 int dense_device_status(int reset);
+int linear_device_status(int reset);
 int dense_set_wait_budget(long long cycles);
+int linear_set_wait_budget(long long cycles);
 int f16_set_wait_budget(long long cycles);
 int peer_set_wait_budget(long long cycles);
 int gemv_tc_set_wait_budget(long long cycles);
@@ -657,6 +659,7 @@ extern "C" int hb200_set_wait_budget_cycles(int64_t cycles) {
   if (rc == HB200_OK) rc = gemv_tc_set_wait_budget(cycles);
   if (rc == HB200_OK) rc = fp8_set_wait_budget(cycles);
   if (rc == HB200_OK) rc = dense_set_wait_budget(cycles);
+  if (rc == HB200_OK) rc = linear_set_wait_budget(cycles);
   return rc;
 }
 
@@ -680,5 +683,6 @@ extern "C" int hb200_device_status(int reset) {
   const int t = hb200::gemv_tc_device_status(reset);
   const int f = hb200::fp8_device_status(reset);
   const int d = hb200::dense_device_status(reset);
-  return v != 0 ? v : (w != 0 ? w : (p != 0 ? p : (t != 0 ? t : (f != 0 ? f : d))));
+  const int l = hb200::linear_device_status(reset);
+  return v != 0 ? v : (w != 0 ? w : (p != 0 ? p : (t != 0 ? t : (f != 0 ? f : (d != 0 ? d : l)))));
 }

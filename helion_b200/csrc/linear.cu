@@ -1,0 +1,457 @@
+// Linear layer with its epilogue fused, for sm_100a (tcgen05 kind::f16, fp32 accumulate; bf16 or fp16 operands):
+//   y[m, n] = cast( act(x[m, :] . w[n, :] + bias[n]) + residual[m, n] )
+// and, gated, with the weight's rows split into a gate half [0, N) and an up half [N, 2 N):
+//   y[m, n] = cast( act(x . w[n] + bias[n]) * (x . w[N + n] + bias[N + n]) + residual[m, n] ).
+// Everything between the accumulator and the one final rounding happens in fp32.
+//
+// linear_stream_kernel streams the WEIGHT through the tensor core's M side: a tile is 128 weight rows (64 gate and 64
+// up rows when gated) by up to 256 rows of x, and the accumulator holds y transposed (lane = weight row, column =
+// row of x).  A decode step is bound by the weight's bytes, and one SM streams about 1/148 of the HBM bandwidth, so
+// the K range of a tile is split over a thread-block cluster of 1, 2, 4 or 8 CTAs until there are enough CTAs for the
+// SMs.  The partial sums meet in distributed shared memory: column c of the tile belongs to rank c % split, every
+// rank stores its fp32 partial of a column into the owner's shared memory, and after one cluster barrier the owner
+// adds them in rank order (ascending K: the result does not depend on timing) and runs the epilogue.  No workspace,
+// no counters, no atomics: calls on any streams and replays of any graphs are independent of each other.
+//
+// CTAs of 192 threads: warp 0 TMA producer (128-byte swizzle, no multicast), warp 1 MMA issuer, warps 2-5 move the
+// accumulator out of tensor memory; all six run the epilogue.  Every wait is bounded.
+#include "gemm_common.cuh"
+
+#include <type_traits>
+
+namespace hb200 {
+
+__device__ int g_device_status_linear = 0;
+
+namespace linear {
+
+using namespace sm100;
+
+enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3, kGeluTanh = 4 };
+
+struct Args {
+  void* out;             // [M, N], row pitch ldo
+  const void* bias;      // [weight rows] in the operand type or (bias_f32) fp32, or nullptr
+  const void* residual;  // [M, N] in the output type, row pitch ldr, or nullptr
+  int64_t ldo, ldr;
+  int m, n, k;           // n: output columns (the weight has 2 n rows when gated)
+  int activation;
+  int bias_f32;
+  int out_vec, res_vec;  // 16-byte accesses are possible
+  int cols, m_chunks;    // rows of x per tile (a multiple of 16), tiles along M
+  int num_kb;            // K blocks of 64 elements
+  int split_log;         // log2 of the CTAs per tile (cluster size)
+  int stages, stage_bytes;
+  int stash_offset;      // bytes from the ring's start to the partial sums (0: they take the ring's place)
+};
+
+// ------------------------------------------------------------------ epilogue arithmetic
+// The fast exponential and division are off by a few units in the last place of fp32, far less than what fp32
+// accumulation of K products leaves in v itself; a divisor beyond 2^126 gives 0, as it should.
+__device__ __forceinline__ float activate(float v, int activation) {
+  switch (activation) {
+    case kRelu: return v > 0.f ? v : (v != v ? v : 0.f);  // a NaN stays a NaN
+    case kSilu: return __fdividef(v, 1.f + __expf(-v));
+    case kGelu: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    case kGeluTanh: {
+      // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u))
+      const float u = 0.79788456080286536f * v * fmaf(0.044715f * v, v, 1.f);
+      return __fdividef(v, 1.f + __expf(-2.f * u));
+    }
+    default: return v;
+  }
+}
+
+template <typename T> __device__ __forceinline__ T cast_out(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 cast_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half cast_out<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ float cast_out<float>(float v) { return v; }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float widen(float v) { return v; }
+
+template <typename T>
+__device__ __forceinline__ float load_bias(const Args& g, int64_t i) {
+  return g.bias_f32 ? static_cast<const float*>(g.bias)[i] : widen(static_cast<const T*>(g.bias)[i]);
+}
+
+// Eight consecutive values of a row: one or two 16-byte accesses where alignment allows.
+template <typename OutT>
+__device__ __forceinline__ void load8(const OutT* p, int valid, bool vec, float (&v)[8]) {
+  if (vec && valid >= 8) {
+    OutT t[8];
+    constexpr int kPieces = int(sizeof(OutT)) / 2;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = widen(t[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < valid ? widen(p[j]) : 0.f;
+  }
+}
+
+template <typename OutT>
+__device__ __forceinline__ void store8(OutT* p, int valid, bool vec, const float (&v)[8]) {
+  if (vec && valid >= 8) {
+    OutT t[8];
+    constexpr int kPieces = int(sizeof(OutT)) / 2;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = cast_out<OutT>(v[j]);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < valid) p[j] = cast_out<OutT>(v[j]);
+  }
+}
+
+// ------------------------------------------------------------------ tensor core
+__device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// kind::f16: fp32 accumulator (bits 4-5 = 1), operand format 0 = f16 / 1 = bf16 at bits 7-9 and 10-12 (both operands
+// alike), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
+__host__ __device__ constexpr uint32_t make_idesc(int m, int n, bool bf16) {
+  return (1u << 4) | (uint32_t(bf16 ? 1 : 0) << 7) | (uint32_t(bf16 ? 1 : 0) << 10) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+// A kernel that gave up a wait lets its own loads land before it leaves: `issued` stages were requested in order.
+__device__ __forceinline__ void drain_loads(uint64_t* full_bar, int stages, int issued) {
+  const long long t0 = clock64();
+  for (int it = issued > stages ? issued - stages : 0; it < issued; ++it)
+    while (!mbar_try_wait(smem_u32(&full_bar[it % stages]), (it / stages) & 1) && clock64() - t0 < 20000000) {}
+}
+
+// ------------------------------------------------------------------ streaming kernel
+constexpr int kStreamThreads = 192;
+constexpr int kTileRows = 128;                 // weight rows per tile
+constexpr int kWBytes = kTileRows * 128;       // one stage of weights: 128 rows x 64 elements
+constexpr int kMaxCols = 256;
+constexpr int kMaxStages = 12;
+constexpr int kBarBytes = 256;
+constexpr int kMaxSplit = 8;
+
+template <typename T, typename OutT, bool GATED>
+__global__ void __launch_bounds__(kStreamThreads)
+linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Args g) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kOutRows = GATED ? 64 : 128;  // output columns per tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(base);
+  uint64_t* empty_bar = full_bar + kMaxStages;
+  uint64_t* done_bar = empty_bar + kMaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* ring = base + 1024;
+  float* stash = reinterpret_cast<float*>(ring + g.stash_offset);  // [rank][column of mine][128] partial sums
+  const bool overlay = g.stash_offset == 0;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split_log = g.split_log, split = 1 << split_log, rank = int(cluster_ctarank());
+  const int tile = int(blockIdx.x) >> split_log;
+  const int m0 = (tile % g.m_chunks) * g.cols, n0 = (tile / g.m_chunks) * kOutRows;
+  const int kb0 = range_start(rank, g.num_kb, split), kb1 = range_start(rank + 1, g.num_kb, split);
+  const int per = g.cols >> split_log;             // columns this rank owns
+  const int live_cols = min(g.cols, g.m - m0); // columns past the last row of x are never stored
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.stages; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    mbar_init(smem_u32(done_bar), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+  }
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < uint32_t(g.cols)) tmem_cols *= 2;
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), tmem_cols);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // A CTA's shared memory may be written by its peers once it runs (or, where the partial sums take the ring's
+  // place, once its MMAs have read the ring): arrive here or below, wait in front of the first remote store.
+  if (!overlay) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+
+  if (warp == 0) {
+    const uint32_t bytes = uint32_t(kWBytes + g.cols * 128);
+    int it = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      const int s = it % g.stages;
+      if (!mbar_wait(smem_u32(&empty_bar[s]), ((it / g.stages) & 1) ^ 1, abort_flag)) break;
+      if (elect_one()) {
+        const uint32_t bar = smem_u32(&full_bar[s]);
+        uint8_t* st = ring + s * g.stage_bytes;
+        mbar_arrive_expect_tx(bar, bytes);
+        tma_load_2d(smem_u32(st), &tmap_w, kb * 64, n0, bar);
+        if constexpr (GATED) tma_load_2d(smem_u32(st + kWBytes / 2), &tmap_w, kb * 64, g.n + n0, bar);
+        tma_load_2d(smem_u32(st + kWBytes), &tmap_x, kb * 64, m0, bar);
+      }
+      __syncwarp();
+    }
+    if (*abort_flag) drain_loads(full_bar, g.stages, it);
+  } else if (warp == 1) {
+    const uint32_t idesc = make_idesc(kTileRows, g.cols, kBf16);
+    bool ok = true;
+    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+      const int s = it % g.stages;
+      if (!mbar_wait(smem_u32(&full_bar[s]), (it / g.stages) & 1, abort_flag)) { ok = false; break; }
+      tcgen05_fence_after();
+      uint8_t* st = ring + s * g.stage_bytes;
+      const uint32_t w_addr = smem_u32(st), x_addr = smem_u32(st + kWBytes);
+      const int k_left = g.k - kb * 64;
+      const int steps = k_left >= 64 ? 4 : (k_left + 15) / 16;  // K tail: TMA zero-fills past K
+      if (elect_one()) {
+        for (int a = 0; a < steps; ++a) {
+          const uint64_t wdesc = make_smem_desc(w_addr + a * 32, 16, 1024, kSwizzle128B);
+          const uint64_t xdesc = make_smem_desc(x_addr + a * 32, 16, 1024, kSwizzle128B);
+          mma_f16(tmem_base, wdesc, xdesc, idesc, (kb != kb0 || a != 0) ? 1u : 0u);
+        }
+        tcgen05_commit(smem_u32(&empty_bar[s]));
+      }
+      __syncwarp();
+    }
+    if (ok && elect_one()) tcgen05_commit(smem_u32(done_bar));
+    __syncwarp();
+  } else {
+    mbar_wait(smem_u32(done_bar), 0, abort_flag);
+    tcgen05_fence_after();
+  }
+  __syncwarp();
+  if (overlay) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+  if (warp >= 2) {
+    const int quarter = warp & 3;
+    const int r_in = quarter * 32 + lane;  // weight row inside the tile = accumulator lane
+    const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16);
+    const uint32_t mine = smem_u32(stash) + uint32_t((rank * per) * 128 + r_in) * 4u;
+#pragma unroll 1
+    for (int c0 = 0; c0 < live_cols; c0 += 8) {
+      uint32_t r[8];
+      tmem_ld_32x32b_x8(taddr + c0, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = c0 + j;
+        if (c < live_cols) st_cluster_f32(map_to_cta(mine + uint32_t(c >> split_log) * 512u, uint32_t(c & (split - 1))), __uint_as_float(r[j]));
+      }
+    }
+    tcgen05_fence_before();
+  }
+  __syncwarp();
+  // Orders the remote stores before the loads below; after it nobody touches another CTA's shared memory again.
+  cluster_sync_all();
+
+  // my i-th column is the tile's column i * split + rank; an item is eight consecutive outputs of one column
+  constexpr int kItemsPerCol = kOutRows / 8;
+  for (int item = threadIdx.x; item < per * kItemsPerCol; item += kStreamThreads) {
+    const int i = item / kItemsPerCol, piece = (item % kItemsPerCol) * 8;
+    const int row = m0 + (i << split_log) + rank, col = n0 + piece;
+    const int valid = g.n - col;
+    if (row >= g.m || valid <= 0) continue;
+    float res[8], acc[8], up[8];
+    if (g.residual != nullptr)
+      load8(static_cast<const OutT*>(g.residual) + int64_t(row) * g.ldr + col, valid, g.res_vec != 0, res);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = up[j] = 0.f;
+    for (int q = 0; q < split; ++q) {
+      const float4* src = reinterpret_cast<const float4*>(stash + (q * per + i) * 128 + piece);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 v = src[h];
+        acc[4 * h] += v.x, acc[4 * h + 1] += v.y, acc[4 * h + 2] += v.z, acc[4 * h + 3] += v.w;
+        if constexpr (GATED) {
+          const float4 w = src[16 + h];
+          up[4 * h] += w.x, up[4 * h + 1] += w.y, up[4 * h + 2] += w.z, up[4 * h + 3] += w.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (g.bias != nullptr && j < valid) {
+        acc[j] += load_bias<T>(g, col + j);
+        if constexpr (GATED) up[j] += load_bias<T>(g, int64_t(g.n) + col + j);
+      }
+      acc[j] = activate(acc[j], g.activation);
+      if constexpr (GATED) acc[j] *= up[j];
+      if (g.residual != nullptr) acc[j] += res[j];
+    }
+    store8(static_cast<OutT*>(g.out) + int64_t(row) * g.ldo + col, valid, g.out_vec != 0, acc);
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem_base, tmem_cols);
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicMin(&g_device_status_linear, HB200_ERR_DEVICE_TIMEOUT);
+}
+
+// ------------------------------------------------------------------ host side
+// K-major 2-byte matrix [rows, K] with a row pitch of `pitch` elements; box = 64 elements (128 bytes) x box_rows.
+bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t pitch, int box_rows, bool bf16) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {cuuint64_t(k), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(pitch) * 2};
+  const cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
+            dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int device_sms() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms > 0 ? sms : 148;
+}
+
+struct StreamPlan {
+  int cols, m_chunks, num_kb, split, split_log, stages, stage_bytes, stash_offset;
+  int64_t tiles;
+  size_t smem;
+};
+
+// Shared memory decides how many CTAs share an SM, and tensor memory must never run short while they do (a CTA that
+// waits for columns could hold up its cluster peers): narrow tiles (at most 64 columns) get half an SM, wider ones a
+// whole SM.
+StreamPlan plan_stream(int64_t m, int64_t n, int64_t k, bool gated, int sms) {
+  StreamPlan p{};
+  p.cols = m >= kMaxCols ? kMaxCols : int((m + 15) / 16 * 16);
+  p.m_chunks = int((m + p.cols - 1) / p.cols);
+  p.num_kb = int((k + 63) / 64);
+  const int out_rows = gated ? 64 : 128;
+  p.tiles = ((n + out_rows - 1) / out_rows) * p.m_chunks;
+  const bool narrow = p.cols <= 64;
+  const int slots = narrow ? 2 * sms : sms;
+  p.split = 1;
+  while (p.split < kMaxSplit && p.tiles * p.split * 2 <= slots && p.num_kb >= 8 * p.split) p.split *= 2, ++p.split_log;
+  p.stage_bytes = kWBytes + ((p.cols * 128 + 1023) / 1024) * 1024;
+  const int budget = (narrow ? 113 : 227) * 1024 - 2048;  // less barriers and alignment
+  const int stash = p.cols * 512;
+  const int fit_beside = (budget - stash) / p.stage_bytes;
+  const bool beside = narrow;  // wide tiles: the partial sums take the ring's place once it has been read
+  p.stages = beside ? fit_beside : budget / p.stage_bytes;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.stash_offset = beside ? p.stages * p.stage_bytes : 0;
+  const int body = beside ? p.stages * p.stage_bytes + stash : (p.stages * p.stage_bytes > stash ? p.stages * p.stage_bytes : stash);
+  p.smem = size_t(body) + 2048;
+  const size_t floor = size_t(narrow ? 77 : 116) * 1024;
+  if (p.smem < floor) p.smem = floor;
+  return p;
+}
+
+template <typename T, typename OutT, bool GATED>
+int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Args& g, const StreamPlan& p, cudaStream_t stream) {
+  auto kernel = linear_stream_kernel<T, OutT, GATED>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(p.smem)) != cudaSuccess) return HB200_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.tiles * p.split), 1, 1);
+  cfg.blockDim = dim3(kStreamThreads, 1, 1);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(p.split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, tw, tx, g) != cudaSuccess) return HB200_ERR_CUDA;
+  return HB200_OK;
+}
+
+template <typename T>
+int launch_stream_typed(const CUtensorMap& tw, const CUtensorMap& tx, const Args& g, const StreamPlan& p, bool gated,
+                        bool out_f32, cudaStream_t s) {
+  if (gated) return out_f32 ? launch_stream<T, float, true>(tw, tx, g, p, s) : launch_stream<T, T, true>(tw, tx, g, p, s);
+  return out_f32 ? launch_stream<T, float, false>(tw, tx, g, p, s) : launch_stream<T, T, false>(tw, tx, g, p, s);
+}
+
+}  // namespace linear
+
+// Wait budget and sticky status of this translation unit (see hb200_set_wait_budget_cycles, hb200_device_status).
+int linear_set_wait_budget(long long cycles) { return sm100::set_wait_budget_cycles(cycles) ? HB200_OK : HB200_ERR_CUDA; }
+
+int linear_device_status(int reset) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_device_status_linear, sizeof(int)) != cudaSuccess) return HB200_ERR_CUDA;
+  if (reset && v != 0) {
+    const int zero = 0;
+    if (cudaMemcpyToSymbol(g_device_status_linear, &zero, sizeof(int)) != cudaSuccess) return HB200_ERR_CUDA;
+  }
+  return v;
+}
+
+}  // namespace hb200
+
+extern "C" int hb200_linear(const void* x, const void* weight, const void* bias, const void* residual, void* out, int64_t m,
+                            int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldo, int activation,
+                            int gated, int is_bf16, int bias_f32, int out_f32, void* stream) {
+  using namespace hb200;
+  using namespace hb200::linear;
+  if (!x || !weight || !out || m <= 0 || n <= 0 || k <= 0 || ldx < k || ldw < k || ldo < n || (residual && ldr < 0))
+    return HB200_ERR_INVALID_ARGUMENT;
+  if (activation < kNone || activation > kGeluTanh) return HB200_ERR_INVALID_ARGUMENT;
+  // TMA: 16-byte aligned bases and row pitches
+  if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(weight) % 16 || (k % 8) != 0 || (ldx % 8) != 0 ||
+      (ldw % 8) != 0)
+    return HB200_ERR_UNSUPPORTED;
+  if (m > 0x3fffff00 || n > 0x3fffff00 || k > 0x3fffff00 || ldx > (int64_t(1) << 38) || ldw > (int64_t(1) << 38))
+    return HB200_ERR_UNSUPPORTED;
+  const int out_size = out_f32 ? 4 : 2;
+  const uintptr_t item = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual);
+  if (item % out_size || reinterpret_cast<uintptr_t>(bias) % (bias_f32 ? 4 : 2)) return HB200_ERR_INVALID_ARGUMENT;
+  const StreamPlan p = plan_stream(m, n, k, gated != 0, device_sms());
+  if (p.tiles * p.split > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
+  CUtensorMap tw, tx;
+  if (!make_map(&tw, weight, gated ? 2 * n : n, k, ldw, gated ? 64 : 128, is_bf16 != 0)) return HB200_ERR_CUDA;
+  if (!make_map(&tx, x, m, k, ldx, p.cols, is_bf16 != 0)) return HB200_ERR_CUDA;
+  Args g{};
+  g.out = out;
+  g.bias = bias;
+  g.residual = residual;
+  g.ldo = ldo;
+  g.ldr = ldr;
+  g.m = int(m);
+  g.n = int(n);
+  g.k = int(k);
+  g.activation = activation;
+  g.bias_f32 = bias_f32 != 0;
+  g.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * out_size) % 16 == 0;
+  g.res_vec = reinterpret_cast<uintptr_t>(residual) % 16 == 0 && (ldr * out_size) % 16 == 0;
+  g.cols = p.cols;
+  g.m_chunks = p.m_chunks;
+  g.num_kb = p.num_kb;
+  g.split_log = p.split_log;
+  g.stages = p.stages;
+  g.stage_bytes = p.stage_bytes;
+  g.stash_offset = p.stash_offset;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return is_bf16 ? launch_stream_typed<__nv_bfloat16>(tw, tx, g, p, gated != 0, out_f32 != 0, s)
+                 : launch_stream_typed<__half>(tw, tx, g, p, gated != 0, out_f32 != 0, s);
+}

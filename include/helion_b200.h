@@ -429,6 +429,19 @@ int hb200_tp_reduce_partials(const void* partials_f32, void* out_bf16, int64_t w
 int hb200_dense_matmul(const void* a, const void* b, void* c, int64_t m, int64_t n, int64_t k, int64_t lda,
                        int64_t ldb, int64_t ldc, int is_bf16, void* stream);
 
+/* Linear layer with its epilogue fused: out [M, N] = cast(act(x . weight^T + bias) + residual), x [M, K] and weight
+ * K-major, both bf16 (is_bf16 != 0) or fp16, fp32 accumulate, everything before the one final rounding in fp32.
+ * activation 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf), 4 GELU (tanh).  gated == 0: weight [N, K], bias [N].  gated != 0:
+ * weight [2 N, K] and bias [2 N] hold N gate rows, then N up rows, and out = cast(act(gate) * up + residual).  bias
+ * (optional) in the operand type or fp32 (bias_f32 != 0); residual (optional) and out in the operand type or fp32
+ * (out_f32 != 0).  Pitches in elements; ldr may be 0 (one row for all).  Any M, N >= 1; K % 8 == 0, 16-byte aligned x
+ * and weight, ldx % 8 == ldw % 8 == 0 (HB200_ERR_UNSUPPORTED otherwise).  No workspace.  residual may be out itself
+ * (same pitch).  No counterpart in the reference (its examples fuse an epilogue into a matmul through a Python
+ * callable). */
+int hb200_linear(const void* x, const void* weight, const void* bias, const void* residual, void* out, int64_t m,
+                 int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldo, int activation, int gated,
+                 int is_bf16, int bias_f32, int out_f32, void* stream);
+
 /* All-gather + matmul (helion_all_gather_matmul, examples/distributed/all_gather_matmul.py:145-196):
  * c [world * rows_local, N] = gathered a . b^T.  a_shard: this rank's rows [rows_local, K], contiguous.
  * gather_ptrs[i] / progress_ptrs[i]: rank i's gather buffer [world * rows_local, K] (contiguous) and its progress

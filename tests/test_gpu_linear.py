@@ -1,0 +1,182 @@
+"""The fused linear layer against its formula in 64 bits: types, activations, odd sizes, strides, streams, graphs."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import helion_b200 as hb
+from helion_b200 import _lib
+from linear_reference import GATED
+from linear_reference import check
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh", *GATED)
+
+
+def make(m, n, k, dtype=torch.bfloat16, activation="none", bias=None, residual=False, out=None, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed + m + 3 * n + 7 * k)
+
+    def normal(*shape, dt, std=1.0):
+        return (torch.randn(*shape, generator=g, device=DEV) * std).to(dt)
+
+    rows = 2 * n if activation in GATED else n
+    out = out or dtype
+    return dict(
+        x=normal(m, k, dt=dtype), weight=normal(rows, k, dt=dtype, std=k**-0.5),
+        bias=None if bias is None else normal(rows, dt=bias, std=0.5),
+        residual=normal(m, n, dt=out) if residual else None, activation=activation,
+    ), out
+
+
+def call(a, out):
+    return hb.linear(a["x"], a["weight"], a["bias"], activation=a["activation"], residual=a["residual"], out_dtype=out)
+
+
+def status_ok():
+    torch.cuda.synchronize()
+    return _lib.load().hb200_device_status(1) == 0
+
+
+# one row, a decode batch, tile edges, several tiles, both sides of every size at which another form takes over
+SIZES = [
+    (1, 1, 8), (1, 128, 4096), (1, 1000, 136), (2, 3, 16), (7, 5001, 72), (15, 130, 1032), (16, 64, 64), (17, 257, 520),
+    (33, 127, 24), (64, 128, 2048), (65, 200, 264), (129, 96, 1032), (200, 640, 2048), (256, 256, 128), (257, 129, 136),
+    (300, 1000, 1064), (513, 264, 72), (1003, 499, 520), (5, 8, 16384), (128, 8, 8192), (383, 512, 512), (640, 2048, 256),
+]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("activation", ["none", "silu_and_mul"])
+def test_sizes(m, n, k, activation):
+    a, out = make(m, n, k, activation=activation, residual=True)
+    y = call(a, out)
+    assert status_ok()
+    check(y, **a)
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(3, 77, 128), (70, 264, 640), (700, 520, 264)])
+def test_activations_and_types(m, n, k, dtype, activation):
+    for bias, residual, out in ((None, False, dtype), (dtype, True, dtype), (torch.float32, True, torch.float32)):
+        a, out = make(m, n, k, dtype, activation, bias, residual, out)
+        y = call(a, out)
+        assert y.dtype is out and status_ok()
+        check(y, **a)
+
+
+@pytest.mark.parametrize("m", [1, 40, 600])
+def test_strides_and_shapes(m):
+    a, out = make(m, 136, 256, bias=torch.bfloat16, residual=True)
+    want = call(a, out)
+    wide = torch.full((m, 256 + 72), float("nan"), dtype=torch.bfloat16, device=DEV)
+    wide[:, 8:264] = a["x"]
+    assert torch.equal(call({**a, "x": wide[:, 8:264]}, out), want)  # a slice with a pitch, read in place
+    wide[:, 3:259] = a["x"]
+    assert torch.equal(call({**a, "x": wide[:, 3:259]}, out), want)  # rows off the 16-byte grid
+    assert torch.equal(call({**a, "x": a["x"].t().contiguous().t()}, out), want)
+    assert torch.equal(call({**a, "weight": a["weight"].t().contiguous().t()}, out), want)
+    tall = torch.full((137, 264), float("nan"), dtype=torch.bfloat16, device=DEV)
+    tall[1:, :256] = a["weight"]
+    assert torch.equal(call({**a, "weight": tall[1:, :256]}, out), want)
+    res = torch.full((m, 150), float("nan"), dtype=torch.bfloat16, device=DEV)
+    res[:, 5:141] = a["residual"]
+    assert torch.equal(call({**a, "residual": res[:, 5:141]}, out), want)
+    assert torch.equal(call({**a, "residual": a["residual"].t().contiguous().t()}, out), want)
+    assert torch.equal(call({**a, "bias": torch.stack([a["bias"], a["bias"]], 1)[:, 1]}, out), want)
+    one = a["residual"][:1].expand(m, -1)  # one residual row for all
+    check(call({**a, "residual": one}, out), **{**a, "residual": one})
+    same = a["x"][:1].expand(m, -1)  # one row of x for all
+    check(call({**a, "x": same}, out), **{**a, "x": same})
+    if m % 2 == 0:
+        y = hb.linear(a["x"].view(2, m // 2, 256), a["weight"], a["bias"], residual=a["residual"].view(2, m // 2, 136))
+        assert torch.equal(y.view(m, 136), want)
+    assert torch.equal(hb.linear(a["x"][0], a["weight"]), hb.linear(a["x"][:1], a["weight"])[0])
+    assert status_ok()
+
+
+def test_empty():
+    w = torch.zeros(24, 64, dtype=torch.float16, device=DEV)
+    assert hb.linear(torch.zeros(0, 64, dtype=torch.float16, device=DEV), w).shape == (0, 24)
+    assert hb.linear(torch.zeros(5, 0, 64, dtype=torch.float16, device=DEV), w, activation="silu_and_mul").shape == (5, 0, 12)
+    assert hb.linear(torch.zeros(3, 64, dtype=torch.float16, device=DEV), w[:0]).shape == (3, 0)
+
+
+@pytest.mark.parametrize("m", [2, 500])
+def test_infinities_and_nan_stay_in_their_rows_and_columns(m):
+    a, out = make(m, 300, 264)
+    clean = call(a, out)
+    a["x"][1, 5] = float("nan")
+    a["weight"][7, 100] = float("inf")
+    y = call(a, out)
+    assert torch.isnan(y[1]).all()
+    rows = torch.arange(m, device=DEV) != 1
+    cols = torch.arange(300, device=DEV) != 7
+    assert torch.equal(y[rows][:, cols], clean[rows][:, cols])
+    assert not torch.isfinite(y[:, 7]).any()
+    relu = call({**a, "activation": "relu"}, out)
+    assert torch.isnan(relu[1]).all()
+
+
+def test_rows_past_the_edges_are_not_written_and_calls_repeat():
+    lib = _lib.load()
+    for m, n, k in ((3, 100, 64), (270, 300, 72)):
+        a, _ = make(m, n, k)
+        ldo = n + 20
+        out = torch.full((m + 2, ldo), 7.0, dtype=torch.bfloat16, device=DEV)
+        for _ in range(2):
+            rc = lib.hb200_linear(a["x"].data_ptr(), a["weight"].data_ptr(), None, None, out[1:].data_ptr(), m, n, k, k, k, 0,
+                                  ldo, 0, 0, 1, 0, 0, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0 and status_ok()
+            assert torch.equal(out[1 : m + 1, :n], call(a, torch.bfloat16))
+            assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[:, n:] == 7).all()
+        # the residual may be the output itself
+        res = torch.randn(m, ldo, device=DEV).to(torch.bfloat16)
+        want = hb.linear(a["x"], a["weight"], residual=res[:, :n])
+        rc = lib.hb200_linear(a["x"].data_ptr(), a["weight"].data_ptr(), None, res.data_ptr(), res.data_ptr(), m, n, k, k, k,
+                              ldo, ldo, 0, 0, 1, 0, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and status_ok() and torch.equal(res[:, :n], want)
+
+
+def test_streams_and_graphs_are_independent():
+    cases = [make(m, 520, 1024, activation="gelu", residual=True, seed=s) for s, m in enumerate((1, 24, 90, 700))]
+    want = [call(a, out) for a, out in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, (a, out) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(call(a, out))
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for y, w in zip(got, want))
+    graphs = []
+    for a, out in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call(a, out)
+        graphs.append((graph, y))
+    for a, _ in cases:
+        a["x"].mul_(2)  # a replay reads the inputs as they are then
+    want = [call(a, out) for a, out in cases]
+    torch.cuda.synchronize()
+    for s, (graph, _) in zip(streams, graphs):  # replayed at the same time: they share nothing
+        with torch.cuda.stream(s):
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for (_, y), w in zip(graphs, want)) and status_ok()
+
+
+def test_registered_operator_and_inference_only():
+    a, out = make(9, 64, 128, bias=torch.bfloat16)
+    want = call(a, out)
+    assert torch.equal(torch.ops.helion_b200.linear(a["x"], a["weight"], a["bias"], None, "none", out), want)
+    torch.library.opcheck(torch.ops.helion_b200.linear, (a["x"], a["weight"], a["bias"], None, "none", out),
+                          test_utils=("test_schema", "test_faketensor"))
+    w = torch.nn.Parameter(a["weight"])
+    with torch.no_grad():
+        assert torch.equal(hb.linear(a["x"], w, a["bias"]), want)
+    with pytest.raises(RuntimeError):
+        hb.linear(a["x"], w, a["bias"]).float().sum().backward()
