@@ -38,6 +38,8 @@ from .ops import rms_norm_nvfp4_quant
 from .ops import silu_and_mul_nvfp4_quant
 from .ops import rms_norm_per_block_quant
 from .ops import silu_and_mul_per_block_quant
+from .routing import Routing
+from .routing import route_experts
 
 __all__ = [
     "grouped_gemm",
@@ -66,6 +68,8 @@ __all__ = [
     "silu_and_mul_nvfp4_quant",
     "rms_norm_per_block_quant",
     "silu_and_mul_per_block_quant",
+    "Routing",
+    "route_experts",
     "swizzle_fp8_scales",
     "swizzled_scale_numel",
     "swizzled_scale_offsets",

@@ -73,6 +73,7 @@ SIGNATURES: dict[str, list] = {
     "hb200_reduce_slots": [_P, _P, _I64, _I64, _I64, _I64, c_int, _P],
     "hb200_nvfp4_gemv_tc_workspace_bytes": [_I64, _I64, _I64, _I64],
     "hb200_moe_route_top_k": [_P, c_int, _I64, _I64, _I64, _P, _P, _P],
+    "hb200_moe_route_experts": [_P, c_int, _I64, _I64, _I64, _I64, c_int, _P, _I64, _I64, _I64, c_int, c_float, _P, _P, _P],
     "hb200_silu_mul_fp8": [_P, _P, _P, _I64, _I64, _I64, c_int, _P],
     "hb200_fp8_scaled_mm_workspace_bytes": [_I64, _I64, _I64],
     "hb200_fp8_scaled_mm": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, c_int, c_int, c_int, c_int, _P,

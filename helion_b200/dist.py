@@ -541,7 +541,7 @@ def expert_parallel_moe(x: Tensor, router_logits: Tensor, top_k: int, num_expert
     """MoE layer over expert-parallel ranks with the process group's all-to-all as the data plane.
     ``x [T_local, H]`` are this rank's tokens; ``expert_fn`` applies this rank's experts to the rows it receives
     (no routing weight).  Returns bf16 ``[T_local, H]``.  ``router`` and ``combine`` default to the CUDA kernels
-    (``moe.route_top_k``, :func:`combine_rows`); host-logic tests inject tensor-code stand-ins."""
+    (``moe.route_top_k``, :func:`combine_rows`; a :class:`~helion_b200.routing.Routing` is a router too); host-logic tests inject tensor-code stand-ins."""
     if router is None:
         from .moe import route_top_k as router
     if combine is None:
@@ -645,15 +645,16 @@ class ExpertParallel:
             self._tp.barrier()
 
     # -- phases (a rank's phases run in this order; ranks meet at the barriers)
-    def dispatch(self, x: Tensor, router_logits: Tensor) -> None:
-        """Route, quantise every token once, sort the (token, slot) pairs by expert and push them to their ranks."""
+    def dispatch(self, x: Tensor, router_logits: Tensor, routing: Router | None = None) -> None:
+        """Route (``routing``: a :class:`~helion_b200.routing.Routing`; softmax and top-k without one), quantise every
+        token once, sort the (token, slot) pairs by expert and push them to their ranks."""
         from . import _lib
         from . import moe as M
         from . import ops
 
         if x.shape != (self.tokens, self.hidden) or x.dtype is not torch.bfloat16 or not x.is_contiguous():
             raise ValueError(f"x must be a contiguous bfloat16 [{self.tokens}, {self.hidden}] tensor")
-        weights, experts = M.route_top_k(router_logits, self.top_k)
+        weights, experts = (routing or M.route_top_k)(router_logits, self.top_k)
         codes_t, scales_t, g_t = ops.nvfp4_quantize(x)
         flat = experts.reshape(-1)
         pairs = flat.numel()
@@ -735,9 +736,10 @@ class ExpertParallel:
         self._state = None
         return out
 
-    def moe(self, x: Tensor, router_logits: Tensor, w_gate_up, w_down) -> Tensor:
-        """One MoE layer step: ``x [tokens, hidden]`` bf16 and ``router_logits [tokens, E]`` of this rank's tokens."""
-        self.dispatch(x, router_logits)
+    def moe(self, x: Tensor, router_logits: Tensor, w_gate_up, w_down, routing: Router | None = None) -> Tensor:
+        """One MoE layer step: ``x [tokens, hidden]`` bf16 and ``router_logits [tokens, E]`` of this rank's tokens;
+        ``routing`` as in :meth:`dispatch` (the same on every rank)."""
+        self.dispatch(x, router_logits, routing)
         self._barrier()  # every rank's rows, counts and tables have arrived
         self.run_experts(w_gate_up, w_down)
         self._barrier()  # every rank's returned rows have arrived

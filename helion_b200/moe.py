@@ -29,6 +29,7 @@ from .layouts import nvfp4_global_scale
 from .layouts import swizzled_scale_numel
 from .ops import _require_cuda
 from .ops import _stream
+from .routing import Routing
 
 
 @dataclass
@@ -297,24 +298,32 @@ def _quantize_rows_amax(y: Tensor, row_amax: Tensor, k: int, sched: MoeSchedule,
 
 @torch.library.custom_op("helion_b200::nvfp4_moe", mutates_args=())
 def _nvfp4_moe_op(x: Tensor, router_logits: Tensor, top_k: int, gu_packed: Tensor, gu_scales: Tensor,
-                  gu_global: Tensor, gu_interleaved: bool, d_packed: Tensor, d_scales: Tensor, d_global: Tensor) -> Tensor:
+                  gu_global: Tensor, gu_interleaved: bool, d_packed: Tensor, d_scales: Tensor, d_global: Tensor,
+                  scoring: str = "", route_bias: Tensor | None = None, num_groups: int = 1, top_groups: int = 1,
+                  group_top: int = 1, renormalize: bool = False, route_scale: float = 1.0) -> Tensor:
+    # no scoring: softmax and top-k alone (route_top_k)
+    routing = Routing(scoring, route_bias, num_groups, top_groups, group_top, renormalize, route_scale) if scoring else None
     return _nvfp4_moe_impl(x, router_logits, top_k, GroupedNvfp4Weight(gu_packed, gu_scales, gu_global, gu_interleaved),
-                           GroupedNvfp4Weight(d_packed, d_scales, d_global), None)
+                           GroupedNvfp4Weight(d_packed, d_scales, d_global), None, routing)
 
 
 @_nvfp4_moe_op.register_fake
-def _(x, router_logits, top_k, gu_packed, gu_scales, gu_global, gu_interleaved, d_packed, d_scales, d_global):
+def _(x, router_logits, top_k, gu_packed, gu_scales, gu_global, gu_interleaved, d_packed, d_scales, d_global, scoring="",
+      route_bias=None, num_groups=1, top_groups=1, group_top=1, renormalize=False, route_scale=1.0):
     return x.new_empty(x.shape)
 
 
 def nvfp4_moe(x: Tensor, router_logits: Tensor, top_k: int, w_gate_up: GroupedNvfp4Weight,
-              w_down: GroupedNvfp4Weight, *, intermediates: dict | None = None) -> Tensor:
+              w_down: GroupedNvfp4Weight, *, routing: Routing | None = None,
+              intermediates: dict | None = None) -> Tensor:
     """NVFP4 MoE layer: ``x [T, H]`` bf16, ``router_logits [T, E]`` -> bf16 ``[T, H]``
     (``torch.ops.helion_b200.nvfp4_moe`` on the bundles' tensors).
 
     The top-k, NVFP4 form of ``moe_matmul_ogs`` (examples/moe_matmul_ogs.py:31-124): softmax-then-top-k routing
     weights used without renormalisation, per-token NVFP4 activations, SiLU-mul between the two expert GEMMs
-    (gate rows first), routing-weighted sum over the top-k slots in slot order.
+    (gate rows first), routing-weighted sum over the top-k slots in slot order.  ``routing`` (a
+    :class:`~helion_b200.routing.Routing`) routes with ``route_experts`` instead: sigmoid scores, a balance bias,
+    expert groups, renormalised or scaled weights.
 
     ``intermediates`` (a dict, filled in place) receives what the second expert GEMM consumes, for parity
     checks: the routing (``weights``, ``experts``), the schedule (``sched``) and, over the padded row layout,
@@ -330,9 +339,13 @@ def nvfp4_moe(x: Tensor, router_logits: Tensor, top_k: int, w_gate_up: GroupedNv
     if w_gate_up.k != h or w_down.k != inter or w_down.n != h or w_down.experts != e:
         raise ValueError("expert weight shapes do not match the activations")
     if intermediates is not None:
-        return _nvfp4_moe_impl(x, router_logits, top_k, w_gate_up, w_down, intermediates)
-    return _nvfp4_moe_op(x, router_logits, top_k, w_gate_up.packed, w_gate_up.scales, w_gate_up.global_scale,
-                         w_gate_up.gate_up_interleaved, w_down.packed, w_down.scales, w_down.global_scale)
+        return _nvfp4_moe_impl(x, router_logits, top_k, w_gate_up, w_down, intermediates, routing)
+    bundles = (w_gate_up.packed, w_gate_up.scales, w_gate_up.global_scale, w_gate_up.gate_up_interleaved, w_down.packed,
+               w_down.scales, w_down.global_scale)
+    if routing is None:
+        return _nvfp4_moe_op(x, router_logits, top_k, *bundles)
+    return _nvfp4_moe_op(x, router_logits, top_k, *bundles, routing.scoring, routing.bias, routing.num_groups,
+                         routing.top_groups, routing.group_top, routing.renormalize, routing.scale)
 
 
 def _row_padding(pairs: int, experts: int, n1: int, n2: int) -> int:
@@ -346,11 +359,11 @@ def _row_padding(pairs: int, experts: int, n1: int, n2: int) -> int:
 
 
 def _nvfp4_moe_impl(x: Tensor, router_logits: Tensor, top_k: int, w_gate_up: GroupedNvfp4Weight,
-                    w_down: GroupedNvfp4Weight, intermediates: dict | None) -> Tensor:
+                    w_down: GroupedNvfp4Weight, intermediates: dict | None, routing: Routing | None = None) -> Tensor:
     t, h = x.shape
     e = w_gate_up.experts
     inter = w_gate_up.n // 2
-    weights, experts = route_top_k(router_logits, top_k)
+    weights, experts = (routing or route_top_k)(router_logits, top_k)
     sched = build_schedule(experts, e, _row_padding(t * top_k, e, w_gate_up.n, h))
     a1, sf1, g1 = _quantize_and_gather(x, sched, top_k)
     y = None

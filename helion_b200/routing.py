@@ -1,0 +1,136 @@
+"""Routing of tokens to experts beyond softmax-then-top-k: sigmoid scores, a balance bias, groups, renormalised weights."""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .fused_linear import _plain
+from .ops import _require_cuda
+
+_SCORINGS = {"softmax": 0, "sigmoid": 1}
+_LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
+           group_top: int) -> None:
+    if router_logits.dim() != 2:
+        raise ValueError("router_logits must be [tokens, experts]")
+    experts = router_logits.shape[1]
+    if router_logits.dtype not in _LOGIT_DTYPES:
+        raise TypeError(f"router_logits must be bfloat16, float16 or float32, got {router_logits.dtype}")
+    if not 1 <= experts <= 1024:
+        raise ValueError(f"1 to 1024 experts are supported, got {experts}")
+    if scoring not in _SCORINGS:
+        raise ValueError(f"scoring must be 'softmax' or 'sigmoid'; got {scoring!r}")
+    if not 1 <= num_groups <= 32 or experts % num_groups:
+        raise ValueError(f"num_groups must be in 1..32 and divide the {experts} experts; got {num_groups}")
+    if not 1 <= top_groups <= num_groups:
+        raise ValueError(f"top_groups must be in 1..{num_groups}, got {top_groups}")
+    size = experts // num_groups
+    if group_top not in (1, 2) or group_top > size:
+        raise ValueError(f"group_top must be 1 or 2 and at most a group's {size} experts; got {group_top}")
+    if not 1 <= top_k <= min(32, top_groups * size):
+        raise ValueError(f"top_k must be in 1..{min(32, top_groups * size)}, got {top_k}")
+    if bias is not None:
+        if bias.shape != (experts,):
+            raise ValueError(f"bias must be [{experts}], got {tuple(bias.shape)}")
+        if bias.dtype is not torch.float32:
+            raise TypeError(f"bias must be float32, got {bias.dtype}")
+        if bias.device != router_logits.device:
+            raise ValueError(f"all tensors must be on one device, got {router_logits.device} and {bias.device}")
+
+
+def _route_cuda(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
+                group_top: int, renormalize: bool, scale: float) -> tuple[Tensor, Tensor]:
+    _check(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top)
+    _require_cuda(router_logits, bias)
+    tokens, experts = router_logits.shape
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=router_logits.device)
+    chosen = torch.empty((tokens, top_k), dtype=torch.int64, device=router_logits.device)
+    if tokens == 0:
+        return weights, chosen
+    if experts > 1 and router_logits.stride(1) != 1:
+        router_logits = router_logits.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    index = router_logits.get_device()
+
+    def launch() -> None:
+        _lib.call(
+            "hb200_moe_route_experts", router_logits.data_ptr(), _LOGIT_DTYPES[router_logits.dtype], tokens, experts,
+            router_logits.stride(0), top_k, _SCORINGS[scoring], None if bias is None else bias.data_ptr(), num_groups,
+            top_groups, group_top, renormalize, scale, weights.data_ptr(), chosen.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(index),
+        )
+
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            launch()
+    else:
+        launch()
+    return weights, chosen
+
+
+@torch.library.custom_op("helion_b200::moe_route_experts", mutates_args=())
+def _route_op(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
+              group_top: int, renormalize: bool, scale: float) -> tuple[Tensor, Tensor]:
+    return _route_cuda(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
+
+
+@_route_op.register_fake
+def _(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale):
+    _check(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top)
+    shape = (router_logits.shape[0], top_k)
+    return router_logits.new_empty(shape, dtype=torch.float32), router_logits.new_empty(shape, dtype=torch.int64)
+
+
+def route_experts(router_logits: Tensor, top_k: int, *, scoring: str = "softmax", bias: Tensor | None = None,
+                  num_groups: int = 1, top_groups: int = 1, group_top: int = 1, renormalize: bool = False,
+                  scale: float = 1.0) -> tuple[Tensor, Tensor]:
+    """Chosen experts of every token and their weights, in one kernel (``torch.ops.helion_b200.moe_route_experts``).
+
+    ``router_logits [T, E]`` in bf16, fp16 or fp32, any row pitch.  Returns ``(weights [T, top_k] fp32, experts
+    [T, top_k] int64)`` in descending order of choice, equal choices by ascending index: what ``moe.build_schedule``
+    and the grouped GEMMs take.
+
+    * score: ``softmax`` over the experts or ``sigmoid`` of each logit, in fp32.
+    * choice: the score plus ``bias [E]`` (fp32, a load-balancing bias); it decides which experts are picked but never
+      enters the weights.
+    * groups: the experts in ``num_groups`` equal runs; a group's score is the sum of its best ``group_top`` (1 or 2)
+      choices, and only the best ``top_groups`` groups' experts can be picked.
+    * weights: the picked experts' scores, divided by their sum with ``renormalize``, times ``scale``.
+
+    The picks are those of exact arithmetic: where two choices are too close for fp32 the row is decided in 64 bits.
+    A logit of ``-inf`` masks an expert: it counts in no sum, is picked only when nothing else is left (ascending
+    index) and gets weight 0; a row with every expert masked gets weights 0.  A row with a NaN (or, under softmax, a
+    logit of ``+inf``) gets NaN weights and distinct experts.  ``E <= 1024``, ``top_k <= 32``, ``num_groups <= 32``.
+    """
+    args = (router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
+    if _plain(router_logits, bias):
+        return _route_cuda(*args)
+    _check(*args[:7])
+    return _route_op(*args)
+
+
+@dataclass(frozen=True)
+class Routing:
+    """The settings of :func:`route_experts` that belong to a model, for the MoE layers that take them
+    (``moe.nvfp4_moe``, ``dist.ExpertParallel``); called with ``(router_logits, top_k)`` it routes, so it also is a
+    router for ``dist.expert_parallel_moe``."""
+
+    scoring: str = "softmax"
+    bias: Tensor | None = None
+    num_groups: int = 1
+    top_groups: int = 1
+    group_top: int = 1
+    renormalize: bool = False
+    scale: float = 1.0
+
+    def __call__(self, router_logits: Tensor, top_k: int) -> tuple[Tensor, Tensor]:
+        return route_experts(router_logits, top_k, scoring=self.scoring, bias=self.bias, num_groups=self.num_groups,
+                             top_groups=self.top_groups, group_top=self.group_top, renormalize=self.renormalize,
+                             scale=self.scale)

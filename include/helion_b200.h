@@ -314,6 +314,19 @@ int hb200_nvfp4_grouped_matmul_256(const void* a_packed, const void* b_packed, c
 int hb200_moe_route_top_k(const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t top_k,
                           float* weights, int64_t* chosen, void* stream);
 
+/* Routing with scores, a balance bias, expert groups and renormalised weights, one kernel.  logits [tokens, experts],
+ * row pitch ld (elements), logits_dtype 0 bf16 / 1 fp16 / 2 fp32; scoring 0 softmax / 1 sigmoid; bias (optional) fp32
+ * [experts], added to the scores for the choice only.  The experts form num_groups equal runs; a group's score is the
+ * sum of its best group_top (1 or 2) choices, the best top_groups groups stay (num_groups = top_groups = 1: no
+ * groups).  weights [tokens, top_k] fp32 = scores of the picks (/ their sum when renormalize != 0) * scale, chosen
+ * [tokens, top_k] int64, in descending order of choice, ties by ascending index.  Logits of -inf are masked experts:
+ * picked last, weight 0; a row with a NaN gets NaN weights and valid indices.  experts <= 1024, top_k <= 32,
+ * num_groups <= 32 and a divisor of experts, top_k <= top_groups * experts / num_groups.  No counterpart in the
+ * reference (see hb200_moe_route_top_k). */
+int hb200_moe_route_experts(const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t ld,
+                            int64_t top_k, int scoring, const float* bias, int64_t num_groups, int64_t top_groups,
+                            int64_t group_top, int renormalize, float scale, float* weights, int64_t* chosen, void* stream);
+
 /* Stable sort of the (token, slot) pairs by expert plus the per-expert counts, on the device: what
  * moe_matmul_ogs_helion_kernel_args_gen computes with bincount + argsort and a host read
  * (examples/moe_matmul_ogs.py:96-117).  expert_of_pair: one entry per pair, int64 when idx_is_i64 != 0 (what

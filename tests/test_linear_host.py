@@ -71,3 +71,73 @@ def test_linear_entry_point_rejects_bad_arguments_before_any_cuda_call():
     assert call(x=p + 2) == unsupported and call(w=p + 8) == unsupported
     assert call(out=p + 1) == bad and call(bias=p + 2, bias_f32=1) == bad and call(res=p + 1) == bad
     assert call(m=1 << 30) == unsupported
+
+
+@pytest.mark.parametrize(
+    "error,match,logits,top_k,kwargs",
+    [
+        (ValueError, "tokens, experts", torch.zeros(8), 2, {}),
+        (TypeError, "bfloat16, float16 or float32", torch.zeros(4, 8, dtype=torch.float64), 2, {}),
+        (ValueError, "1024 experts", torch.zeros(4, 1025), 2, {}),
+        (ValueError, "1024 experts", torch.zeros(4, 0), 1, {}),
+        (ValueError, "scoring", torch.zeros(4, 8), 2, {"scoring": "relu"}),
+        (ValueError, "num_groups", torch.zeros(4, 8), 2, {"num_groups": 3}),
+        (ValueError, "num_groups", torch.zeros(4, 66), 2, {"num_groups": 33}),
+        (ValueError, "num_groups", torch.zeros(4, 8), 2, {"num_groups": 0}),
+        (ValueError, "top_groups", torch.zeros(4, 8), 2, {"num_groups": 4, "top_groups": 5}),
+        (ValueError, "top_groups", torch.zeros(4, 8), 2, {"top_groups": 0}),
+        (ValueError, "group_top", torch.zeros(4, 8), 2, {"num_groups": 4, "group_top": 3}),
+        (ValueError, "group_top", torch.zeros(4, 8), 1, {"num_groups": 8, "group_top": 2}),
+        (ValueError, "top_k", torch.zeros(4, 8), 0, {}),
+        (ValueError, "top_k", torch.zeros(4, 8), 9, {}),
+        (ValueError, "top_k", torch.zeros(4, 64), 33, {}),
+        (ValueError, "top_k", torch.zeros(4, 8), 3, {"num_groups": 4, "top_groups": 1}),
+        (ValueError, "bias must be .8.", torch.zeros(4, 8), 2, {"bias": torch.zeros(7)}),
+        (TypeError, "bias must be float32", torch.zeros(4, 8), 2, {"bias": torch.zeros(8, dtype=torch.bfloat16)}),
+        (ValueError, "one device", torch.zeros(4, 8), 2, {"bias": torch.zeros(8, device="meta")}),
+        (RuntimeError, "no CPU fallback", torch.zeros(4, 8), 2, {}),
+    ],
+)
+def test_route_refusals(error, match, logits, top_k, kwargs):
+    with pytest.raises(error, match=match):
+        hb.route_experts(logits, top_k, **kwargs)
+    with pytest.raises(error, match=match):
+        hb.Routing(**kwargs)(logits, top_k)
+
+
+def test_route_traces_under_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        w, e = hb.route_experts(torch.empty(5, 64, device="cuda", dtype=torch.bfloat16), 6, num_groups=8, top_groups=2)
+        assert w.shape == e.shape == (5, 6) and w.dtype is torch.float32 and e.dtype is torch.int64
+
+
+def test_route_entry_point_rejects_bad_arguments_before_any_cuda_call():
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+
+    def call(logits=p, dtype=2, tokens=4, experts=8, ld=8, k=2, scoring=0, groups=1, top_groups=1, group_top=1, w=p, c=p):
+        return lib.hb200_moe_route_experts(logits, dtype, tokens, experts, ld, k, scoring, None, groups, top_groups, group_top,
+                                           0, 1.0, w, c, None)
+
+    bad = _lib.HB200_ERR_INVALID_ARGUMENT
+    assert call(logits=None) == bad and call(w=None) == bad and call(c=None) == bad
+    assert call(dtype=3) == bad and call(scoring=2) == bad and call(tokens=-1) == bad
+    assert call(experts=0) == bad and call(experts=1025) == bad and call(ld=-1) == bad
+    assert call(k=0) == bad and call(k=9) == bad and call(groups=3) == bad and call(groups=4, top_groups=5) == bad
+    assert call(groups=4, k=3) == bad and call(group_top=3) == bad and call(groups=8, group_top=2, k=1) == bad
+    assert call(tokens=0) == 0
+
+
+def test_reference_router_in_small():
+    """The tests' own reference: values worked out by hand."""
+    from route_reference import route_row
+
+    w, p = route_row([0.0, 2.0, 1.0, -1.0], 2, "softmax", None, 2, 1, 1, True, 1.0)
+    assert p == [1, 0] and abs(w[0] - 1 / (1 + 2.718281828459045**-2)) < 1e-12 and abs(sum(w) - 1) < 1e-12
+    w, p = route_row([0.0, 0.0, 0.0, 0.0], 2, "sigmoid", [0.0, 0.1, 0.1, 0.0], 1, 1, 1, False, 4.0)
+    assert p == [1, 2] and w == [2.0, 2.0]
+    w, p = route_row([float("-inf")] * 4, 3, "softmax", None, 2, 2, 2, True, 1.0)
+    assert p == [0, 1, 2] and w == [0.0, 0.0, 0.0]
