@@ -43,6 +43,9 @@ struct Args {
   int split_log;         // log2 of the CTAs per tile (cluster size)
   int stages, stage_bytes;
   int stash_offset;      // bytes from the ring's start to the partial sums (0: they take the ring's place)
+  // pair kernel
+  int m_tiles, n_tiles;
+  int band;              // row tiles per band of the tile order
 };
 
 // ------------------------------------------------------------------ epilogue arithmetic
@@ -60,6 +63,23 @@ __device__ __forceinline__ float activate(float v, int activation) {
     }
     default: return v;
   }
+}
+
+// The same for an array: one branch on the (uniform) kind in front of the unrolled arithmetic.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&v)[N], int activation) {
+#define HB200_ACTIVATE(kind)                                  \
+  case kind: {                                                \
+    _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = activate(v[j], kind); \
+  } break
+  switch (activation) {
+    HB200_ACTIVATE(kRelu);
+    HB200_ACTIVATE(kSilu);
+    HB200_ACTIVATE(kGelu);
+    HB200_ACTIVATE(kGeluTanh);
+    default: break;
+  }
+#undef HB200_ACTIVATE
 }
 
 template <typename T> __device__ __forceinline__ T cast_out(float v);
@@ -127,6 +147,11 @@ __host__ __device__ constexpr uint32_t make_idesc(int m, int n, bool bf16) {
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+// The bounded wait as one decision of a converged warp: what follows is executed by all of its lanes or by none.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
 // A kernel that gave up a wait lets its own loads land before it leaves: `issued` stages were requested in order.
@@ -199,7 +224,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     int it = 0;
     for (int kb = kb0; kb < kb1; ++kb, ++it) {
       const int s = it % g.stages;
-      if (!mbar_wait(smem_u32(&empty_bar[s]), ((it / g.stages) & 1) ^ 1, abort_flag)) break;
+      if (!warp_wait(smem_u32(&empty_bar[s]), ((it / g.stages) & 1) ^ 1, abort_flag)) break;
       if (elect_one()) {
         const uint32_t bar = smem_u32(&full_bar[s]);
         uint8_t* st = ring + s * g.stage_bytes;
@@ -216,7 +241,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     bool ok = true;
     for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
       const int s = it % g.stages;
-      if (!mbar_wait(smem_u32(&full_bar[s]), (it / g.stages) & 1, abort_flag)) { ok = false; break; }
+      if (!warp_wait(smem_u32(&full_bar[s]), (it / g.stages) & 1, abort_flag)) { ok = false; break; }
       tcgen05_fence_after();
       uint8_t* st = ring + s * g.stage_bytes;
       const uint32_t w_addr = smem_u32(st), x_addr = smem_u32(st + kWBytes);
@@ -235,7 +260,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     if (ok && elect_one()) tcgen05_commit(smem_u32(done_bar));
     __syncwarp();
   } else {
-    mbar_wait(smem_u32(done_bar), 0, abort_flag);
+    warp_wait(smem_u32(done_bar), 0, abort_flag);
     tcgen05_fence_after();
   }
   __syncwarp();
@@ -294,7 +319,10 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         acc[j] += load_bias<T>(g, col + j);
         if constexpr (GATED) up[j] += load_bias<T>(g, int64_t(g.n) + col + j);
       }
-      acc[j] = activate(acc[j], g.activation);
+    }
+    activate_all(acc, g.activation);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
       if constexpr (GATED) acc[j] *= up[j];
       if (g.residual != nullptr) acc[j] += res[j];
     }
@@ -310,6 +338,305 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   if (threadIdx.x == 0 && *abort_flag) atomicMin(&g_device_status_linear, HB200_ERR_DEVICE_TIMEOUT);
 }
 
+// ------------------------------------------------------------------ pair kernel
+// Many rows of x: two CTAs on neighbouring SMs own one tile of 256 rows of x by 256 weight rows (gated: 128 gate rows,
+// held by the leader, and the 128 up rows of the same outputs, held by its peer, so gate and up of an output meet in
+// one accumulator lane 128 columns apart).  CTA r of the pair loads its 128 rows of x and its 128 weight rows, the
+// leader issues 256 x 256 x 16 MMAs (cta_group::2) that read both: per 64 elements of K every SM pulls 32 KB from L2
+// for 512 clocks of tensor work.  Two accumulators in tensor memory, so a tile's epilogue runs beside the next
+// tile's MMAs; the grid is persistent.
+//
+// Epilogue: sixteen warps per CTA, each 32 rows by 64 accumulator columns (gated: 32 gate and 32 up columns).  Outputs
+// pass through a box of 32 rows x 64 bytes per warp in shared memory, and out of it by TMA where the output's pitch
+// allows, else row by row with consecutive lanes on consecutive elements; the residual comes in through the same box
+// the same way, the first one requested before the wait for the accumulator.
+constexpr int kPairThreads = 640;  // producer, MMA issuer, two idle warps, sixteen epilogue warps
+constexpr int kPairTile = 256;
+constexpr int kPairStages = 6;
+constexpr int kHalfBytes = 128 * 128;          // this CTA's 128 rows of x (or of the weight) x 64 elements of K
+constexpr int kPairStageBytes = 2 * kHalfBytes;
+constexpr int kBoxBytes = 2048;
+constexpr int kAcc = 2;
+constexpr size_t kPairSmem = size_t(kPairStages) * kPairStageBytes + 16 * kBoxBytes + (2 * kPairStages + 2 * kAcc) * 8 + 16 + 1024;
+static_assert(kPairSmem <= 232448, "shared memory budget exceeded");
+
+__device__ __forceinline__ void mma_pair_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Bands of `band` row tiles; inside a band the row tile runs fastest: the pairs at work at one time share a few row
+// tiles of x and a few tiles of the weight, which stay in L2.
+__device__ __forceinline__ void decode_tile(const Args& g, int tile, int& m_blk, int& n_blk) {
+  const int per_band = g.band * g.n_tiles;
+  const int b = tile / per_band, r = tile - b * per_band;
+  const int rows_here = min(g.band, g.m_tiles - b * g.band);
+  n_blk = r / rows_here;
+  m_blk = b * g.band + (r - n_blk * rows_here);
+}
+
+// 16-byte chunk c of row r of a box: the 64-byte swizzle of the TMA store.
+__device__ __forceinline__ uint32_t box_chunk(int r, int c) { return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); }
+
+// Residual rows [row0, row0 + 32) x columns [col, col + 64 / size) into a box.
+template <typename OutT>
+__device__ __forceinline__ void fetch_box(const Args& g, uint8_t* box, int row0, int col, int lane) {
+  constexpr int kCols = 64 / int(sizeof(OutT)), kPer = 16 / int(sizeof(OutT));
+  const OutT* src = static_cast<const OutT*>(g.residual);
+  if (g.res_vec && col + kCols <= g.n) {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (row0 + r < g.m) v[i] = *reinterpret_cast<const uint4*>(src + int64_t(row0 + r) * g.ldr + col + (lane & 3) * kPer);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(box + box_chunk(i * 8 + (lane >> 2), lane & 3)) = v[i];
+  } else {
+    constexpr int kRowsAtOnce = 32 / kCols;  // 1 (16-bit) or 2 (fp32)
+    const int c = lane % kCols;
+#pragma unroll 8
+    for (int i = 0; i < 32; i += kRowsAtOnce) {
+      const int r = i + lane / kCols;
+      OutT v = cast_out<OutT>(0.f);
+      if (row0 + r < g.m && col + c < g.n) v = src[int64_t(row0 + r) * g.ldr + col + c];
+      *reinterpret_cast<OutT*>(box + box_chunk(r, c / kPer) + (c % kPer) * sizeof(OutT)) = v;
+    }
+  }
+}
+
+// A box to the output without TMA (a pitch or base off the 16-byte grid): consecutive lanes write consecutive elements.
+template <typename OutT>
+__device__ __forceinline__ void flush_box(const Args& g, const uint8_t* box, int row0, int col, int lane) {
+  constexpr int kCols = 64 / int(sizeof(OutT)), kPer = 16 / int(sizeof(OutT)), kRowsAtOnce = 32 / kCols;
+  OutT* dst = static_cast<OutT*>(g.out);
+  const int c = lane % kCols;
+#pragma unroll 8
+  for (int i = 0; i < 32; i += kRowsAtOnce) {
+    const int r = i + lane / kCols;
+    if (row0 + r < g.m && col + c < g.n)
+      dst[int64_t(row0 + r) * g.ldo + col + c] = *reinterpret_cast<const OutT*>(box + box_chunk(r, c / kPer) + (c % kPer) * sizeof(OutT));
+  }
+}
+
+template <typename T, typename OutT, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                   const __grid_constant__ CUtensorMap tmap_out, const Args g) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kOutCols = GATED ? 128 : 256;           // output columns per tile
+  constexpr int kBoxCols = 64 / int(sizeof(OutT));      // output columns per box
+  constexpr int kBoxesPer32 = 32 / kBoxCols;            // 1 (16-bit outputs) or 2 (fp32)
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* boxes = smem + kPairStages * kPairStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(boxes + 16 * kBoxBytes);  // used in the leader only
+  uint64_t* empty_bar = full_bar + kPairStages;                              // one set per CTA
+  uint64_t* tmem_full_bar = empty_bar + kPairStages;
+  uint64_t* tmem_empty_bar = tmem_full_bar + kAcc;                           // used in the leader only
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty_bar + kAcc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int num_tiles = g.m_tiles * g.n_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);   // the leader's producer arms it; bytes come from both CTAs
+      mbar_init(smem_u32(&empty_bar[s]), 1);  // the leader's commit, sent to both CTAs
+    }
+    for (int a = 0; a < kAcc; ++a) {
+      mbar_init(smem_u32(&tmem_full_bar[a]), 1);
+      mbar_init(smem_u32(&tmem_empty_bar[a]), 32);  // sixteen epilogue warps in each CTA
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // barriers of both CTAs are initialised before anything remote happens
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (both CTAs)
+    int it = 0;
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      int m_blk, n_blk;
+      decode_tile(g, tile, m_blk, n_blk);
+      const int x_row = m_blk * kPairTile + int(rank) * 128;
+      const int w_row = n_blk * kOutCols + int(rank) * (GATED ? g.n : 128);
+      for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
+        const int s = it % kPairStages;
+        if (!warp_wait(smem_u32(&empty_bar[s]), ((it / kPairStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        uint8_t* st = smem + s * kPairStageBytes;
+        const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);  // always the leader's barrier
+        if (elect_one()) {
+          if (leader) mbar_arrive_expect_tx(smem_u32(&full_bar[s]), 2 * kPairStageBytes);
+          tma_load_2d_pair(smem_u32(st), &tmap_x, kb * 64, x_row, bar);
+          tma_load_2d_pair(smem_u32(st + kHalfBytes), &tmap_w, kb * 64, w_row, bar);
+        }
+        __syncwarp();
+      }
+    }
+    if (leader && *abort_flag) drain_loads(full_bar, kPairStages, it);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer (leader only)
+    if (leader) {
+      constexpr uint32_t idesc = make_idesc(256, 256, kBf16);
+      bool ok = true;
+      uint32_t it = 0, tc = 0;
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++tc) {
+        const int acc = tc % kAcc;
+        if (!warp_wait(smem_u32(&tmem_empty_bar[acc]), ((tc / kAcc) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        tcgen05_fence_after();
+        const uint32_t tmem_d = tmem_base + acc * 256;
+        for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
+          const int s = it % kPairStages;
+          if (!warp_wait(smem_u32(&full_bar[s]), (it / kPairStages) & 1, abort_flag)) { ok = false; break; }
+          tcgen05_fence_after();
+          uint8_t* st = smem + s * kPairStageBytes;
+          const uint32_t x_addr = smem_u32(st), w_addr = smem_u32(st + kHalfBytes);
+          const int k_left = g.k - kb * 64;
+          const int steps = k_left >= 64 ? 4 : (k_left + 15) / 16;  // K tail: TMA zero-fills past K
+          if (elect_one()) {
+            for (int a = 0; a < steps; ++a)
+              mma_pair_f16(tmem_d, make_smem_desc(x_addr + a * 32, 16, 1024, kSwizzle128B),
+                           make_smem_desc(w_addr + a * 32, 16, 1024, kSwizzle128B), idesc, (kb | a) != 0 ? 1u : 0u);
+            tcgen05_commit_pair(smem_u32(&empty_bar[s]), 3);  // stage free in both CTAs
+          }
+          __syncwarp();
+        }
+        if (ok && elect_one()) tcgen05_commit_pair(smem_u32(&tmem_full_bar[acc]), 3);
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int quarter = warp & 3, cgroup = (warp - 4) >> 2;  // a warp may read lane quarter warp % 4 only
+    uint8_t* box = boxes + (warp - 4) * kBoxBytes;
+    const bool tma_out = g.out_vec != 0;
+    uint32_t tc = 0;
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++tc) {
+      int m_blk, n_blk;
+      decode_tile(g, tile, m_blk, n_blk);
+      const int acc = tc % kAcc;
+      const int row0 = m_blk * kPairTile + int(rank) * 128 + quarter * 32;
+      const int col0 = n_blk * kOutCols + cgroup * (GATED ? 32 : 64);
+      // the columns' biases: lane l keeps that of column col0 + l of each of the two 32-column blocks
+      float bias_l[2] = {0.f, 0.f};
+      if (g.bias != nullptr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = col0 + (GATED ? 0 : h * 32) + lane;
+          if (c < g.n) bias_l[h] = load_bias<T>(g, c + (GATED && h == 1 ? g.n : 0));
+        }
+      }
+      if (g.residual != nullptr) {
+        if (lane == 0) bulk_wait_group_read0();  // the box's last store has left it
+        __syncwarp();
+        fetch_box<OutT>(g, box, row0, col0, lane);
+      }
+      if (!warp_wait(smem_u32(&tmem_full_bar[acc]), (tc / kAcc) & 1, abort_flag)) { ok = false; break; }
+      tcgen05_fence_after();
+      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * 256 + cgroup * (GATED ? 32 : 64);
+#pragma unroll
+      for (int h = 0; h < (GATED ? 1 : 2); ++h) {
+        uint32_t r[32], u[GATED ? 32 : 1];
+        tmem_ld_32x32b_x32(taddr + h * 32, r);
+        if constexpr (GATED) tmem_ld_32x32b_x32(taddr + 128, reinterpret_cast<uint32_t(&)[32]>(u));
+        tmem_ld_wait();
+        if (GATED || h == 1) {  // everything is in registers: hand the accumulator back
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[acc]), 0));
+        }
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        if (g.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, bias_l[h], j);
+        }
+        activate_all(v, g.activation);
+        if constexpr (GATED) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float up = __uint_as_float(u[j]);
+            if (g.bias != nullptr) up += __shfl_sync(0xffffffffu, bias_l[1], j);
+            v[j] *= up;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kBoxesPer32; ++b) {
+          const int col = col0 + h * 32 + b * kBoxCols;
+          constexpr int kPer = 16 / int(sizeof(OutT));
+          if (h != 0 || b != 0 || g.residual == nullptr) {
+            if (lane == 0) bulk_wait_group_read0();
+            __syncwarp();
+            if (g.residual != nullptr) fetch_box<OutT>(g, box, row0, col, lane);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint4* slot = reinterpret_cast<uint4*>(box + box_chunk(lane, c));
+            OutT o[kPer];
+            if (g.residual != nullptr) {
+              const uint4 raw = *slot;
+              const OutT* res = reinterpret_cast<const OutT*>(&raw);
+#pragma unroll
+              for (int j = 0; j < kPer; ++j) o[j] = cast_out<OutT>(v[b * kBoxCols + c * kPer + j] + widen(res[j]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < kPer; ++j) o[j] = cast_out<OutT>(v[b * kBoxCols + c * kPer + j]);
+            }
+            *slot = *reinterpret_cast<const uint4*>(o);
+          }
+          if (tma_out) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < g.m && col < g.n) {
+              tma_store_2d(&tmap_out, col, row0, smem_u32(box));  // rows and columns past the edge are clipped
+              bulk_commit_group();
+            }
+          } else {
+            __syncwarp();
+            flush_box<OutT>(g, box, row0, col, lane);
+            __syncwarp();
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group_read0();
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer is done with this CTA's shared memory, barriers and tensor memory
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicMin(&g_device_status_linear, HB200_ERR_DEVICE_TIMEOUT);
+}
+
 // ------------------------------------------------------------------ host side
 // K-major 2-byte matrix [rows, K] with a row pitch of `pitch` elements; box = 64 elements (128 bytes) x box_rows.
 bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t pitch, int box_rows, bool bf16) {
@@ -321,6 +648,21 @@ bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64
   const cuuint32_t elem[2] = {1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
             dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Output boxes of the pair kernel: 64 bytes x 32 rows, 64-byte swizzle.
+bool make_out_map(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t pitch, bool f32, bool bf16) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const int size = f32 ? 4 : 2;
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(pitch) * size};
+  const cuuint32_t box[2] = {cuuint32_t(64 / size), 32};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUtensorMapDataType type = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : (bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+  return fn(map, type, 2, base, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -392,6 +734,24 @@ int launch_stream_typed(const CUtensorMap& tw, const CUtensorMap& tx, const Args
   return out_f32 ? launch_stream<T, float, false>(tw, tx, g, p, s) : launch_stream<T, T, false>(tw, tx, g, p, s);
 }
 
+template <typename T, typename OutT, bool GATED>
+int launch_pair(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Args& g, int pairs, cudaStream_t stream) {
+  auto kernel = linear_pair_kernel<T, OutT, GATED>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPairSmem)) != cudaSuccess) return HB200_ERR_CUDA;
+  kernel<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(tw, tx, to, g);
+  return launch_status();
+}
+
+template <typename T>
+int launch_pair_typed(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Args& g, int pairs, bool gated,
+                      bool out_f32, cudaStream_t s) {
+  if (gated) return out_f32 ? launch_pair<T, float, true>(tw, tx, to, g, pairs, s) : launch_pair<T, T, true>(tw, tx, to, g, pairs, s);
+  return out_f32 ? launch_pair<T, float, false>(tw, tx, to, g, pairs, s) : launch_pair<T, T, false>(tw, tx, to, g, pairs, s);
+}
+
+// The pair kernel takes over once its tiles are filled: 384 rows of x and 256 weight rows.
+bool use_pair(int64_t m, int64_t n) { return m >= 384 && n >= 256; }
+
 }  // namespace linear
 
 // Wait budget and sticky status of this translation unit (see hb200_set_wait_budget_cycles, hb200_device_status).
@@ -426,11 +786,9 @@ extern "C" int hb200_linear(const void* x, const void* weight, const void* bias,
   const int out_size = out_f32 ? 4 : 2;
   const uintptr_t item = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual);
   if (item % out_size || reinterpret_cast<uintptr_t>(bias) % (bias_f32 ? 4 : 2)) return HB200_ERR_INVALID_ARGUMENT;
-  const StreamPlan p = plan_stream(m, n, k, gated != 0, device_sms());
-  if (p.tiles * p.split > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
-  CUtensorMap tw, tx;
-  if (!make_map(&tw, weight, gated ? 2 * n : n, k, ldw, gated ? 64 : 128, is_bf16 != 0)) return HB200_ERR_CUDA;
-  if (!make_map(&tx, x, m, k, ldx, p.cols, is_bf16 != 0)) return HB200_ERR_CUDA;
+  const bool bf16 = is_bf16 != 0, f32 = out_f32 != 0, is_gated = gated != 0;
+  const int sms = device_sms();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   Args g{};
   g.out = out;
   g.bias = bias;
@@ -444,14 +802,31 @@ extern "C" int hb200_linear(const void* x, const void* weight, const void* bias,
   g.bias_f32 = bias_f32 != 0;
   g.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * out_size) % 16 == 0;
   g.res_vec = reinterpret_cast<uintptr_t>(residual) % 16 == 0 && (ldr * out_size) % 16 == 0;
+  g.num_kb = int((k + 63) / 64);
+  const int64_t weight_rows = is_gated ? 2 * n : n;
+  CUtensorMap tw, tx, to{};
+  if (use_pair(m, n)) {
+    const int64_t m_tiles = (m + kPairTile - 1) / kPairTile, n_tiles = (weight_rows + kPairTile - 1) / kPairTile;
+    if (m_tiles * n_tiles > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
+    if (!make_map(&tw, weight, weight_rows, k, ldw, 128, bf16) || !make_map(&tx, x, m, k, ldx, 128, bf16)) return HB200_ERR_CUDA;
+    if (g.out_vec && !make_out_map(&to, out, m, n, ldo, f32, bf16)) return HB200_ERR_CUDA;
+    g.m_tiles = int(m_tiles);
+    g.n_tiles = int(n_tiles);
+    g.band = 16;
+    const int pairs = int(m_tiles * n_tiles < sms / 2 ? m_tiles * n_tiles : sms / 2);
+    return bf16 ? launch_pair_typed<__nv_bfloat16>(tw, tx, to, g, pairs, is_gated, f32, s)
+                : launch_pair_typed<__half>(tw, tx, to, g, pairs, is_gated, f32, s);
+  }
+  const StreamPlan p = plan_stream(m, n, k, is_gated, sms);
+  if (p.tiles * p.split > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
+  if (!make_map(&tw, weight, weight_rows, k, ldw, is_gated ? 64 : 128, bf16)) return HB200_ERR_CUDA;
+  if (!make_map(&tx, x, m, k, ldx, p.cols, bf16)) return HB200_ERR_CUDA;
   g.cols = p.cols;
   g.m_chunks = p.m_chunks;
-  g.num_kb = p.num_kb;
   g.split_log = p.split_log;
   g.stages = p.stages;
   g.stage_bytes = p.stage_bytes;
   g.stash_offset = p.stash_offset;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return is_bf16 ? launch_stream_typed<__nv_bfloat16>(tw, tx, g, p, gated != 0, out_f32 != 0, s)
-                 : launch_stream_typed<__half>(tw, tx, g, p, gated != 0, out_f32 != 0, s);
+  return bf16 ? launch_stream_typed<__nv_bfloat16>(tw, tx, g, p, is_gated, f32, s)
+              : launch_stream_typed<__half>(tw, tx, g, p, is_gated, f32, s);
 }

@@ -67,6 +67,19 @@ def test_activations_and_types(m, n, k, dtype, activation):
         check(y, **a)
 
 
+@pytest.mark.parametrize("activation", ["gelu_tanh", "silu_and_mul"])
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("m,n,k", [(9, 333, 72), (90, 131, 200), (433, 387, 328), (1537, 641, 1032)])
+def test_odd_widths_in_every_output_type(m, n, k, dtype, out, activation):
+    a, out = make(m, n, k, dtype, activation, torch.float32, True, out)
+    y = call(a, out)
+    assert status_ok()
+    check(y, **a)
+    wide = torch.full((m, n + 3), float("nan"), dtype=out, device=DEV)
+    wide[:, 2 : 2 + n] = a["residual"]
+    assert torch.equal(call({**a, "residual": wide[:, 2 : 2 + n]}, out), y)
+
+
 @pytest.mark.parametrize("m", [1, 40, 600])
 def test_strides_and_shapes(m):
     a, out = make(m, 136, 256, bias=torch.bfloat16, residual=True)
