@@ -17,6 +17,8 @@
 // accumulator out of tensor memory; all six run the epilogue.  Every wait is bounded.
 #include "gemm_common.cuh"
 
+#include <atomic>
+#include <cstdlib>
 #include <type_traits>
 
 namespace hb200 {
@@ -49,17 +51,42 @@ struct Args {
 };
 
 // ------------------------------------------------------------------ epilogue arithmetic
-// The fast exponential and division are off by a few units in the last place of fp32, far less than what fp32
-// accumulation of K products leaves in v itself; a divisor beyond 2^126 gives 0, as it should.
+// The exponential and the reciprocal are the hardware's approximations, off by two units in the last place of fp32:
+// far less than what fp32 accumulation of K products leaves in v itself.  Their denormals are zero.
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
 __device__ __forceinline__ float activate(float v, int activation) {
   switch (activation) {
     case kRelu: return v > 0.f ? v : (v != v ? v : 0.f);  // a NaN stays a NaN
-    case kSilu: return __fdividef(v, 1.f + __expf(-v));
-    case kGelu: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    case kSilu: return v * reciprocal_fast(1.f + exp2_fast(-kLog2e * v));
+    case kGelu: {
+      // v Phi(v) = max(v, 0) - |v| Phi(-|v|), Phi(-a) = exp(-a^2 / 2) t R(t) with t = 1 / (1 + 0.44 a / sqrt 2): R is a
+      // degree-7 fit of this file's own (weighted least squares on Chebyshev points), off by at most 1.8e-7 of its
+      // value for every a, so the small values of the left tail keep their relative precision
+      const float a = fminf(fabsf(v), 1e4f), t = reciprocal_fast(fmaf(0.31112698f, a, 1.f));
+      float p = fmaf(0.03561173379421234f, t, -0.13897401094436646f);
+      p = fmaf(p, t, 0.1483437418937683f);
+      p = fmaf(p, t, -0.010090325959026814f);
+      p = fmaf(p, t, 0.10790611058473587f);
+      p = fmaf(p, t, 0.10865677893161774f);
+      p = fmaf(p, t, 0.12443558871746063f);
+      p = fmaf(p, t, 0.12411047518253326f);
+      return fmaf(-a, exp2_fast(-0.5f * kLog2e * v * v) * (t * p), fmaxf(v, 0.f));
+    }
     case kGeluTanh: {
-      // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u))
-      const float u = 0.79788456080286536f * v * fmaf(0.044715f * v, v, 1.f);
-      return __fdividef(v, 1.f + __expf(-2.f * u));
+      // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
+      const float u = v * fmaf(-2.f * kLog2e * 0.79788456080286536f * 0.044715f * v, v, -2.f * kLog2e * 0.79788456080286536f);
+      return v * reciprocal_fast(1.f + exp2_fast(u));
     }
     default: return v;
   }
@@ -89,6 +116,15 @@ template <> __device__ __forceinline__ float cast_out<float>(float v) { return v
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ float widen(float v) { return v; }
+
+// Two values of a 16-byte piece, rounded, in one word (fp32: one value).
+template <typename OutT> __device__ __forceinline__ uint32_t pack_word(const float* v);
+template <> __device__ __forceinline__ uint32_t pack_word<__nv_bfloat16>(const float* v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack_word<__half>(const float* v) { return h2_as_u32(__floats2half2_rn(v[0], v[1])); }
+template <> __device__ __forceinline__ uint32_t pack_word<float>(const float* v) { return __float_as_uint(v[0]); }
 
 template <typename T>
 __device__ __forceinline__ float load_bias(const Args& g, int64_t i) {
@@ -167,7 +203,6 @@ constexpr int kTileRows = 128;                 // weight rows per tile
 constexpr int kWBytes = kTileRows * 128;       // one stage of weights: 128 rows x 64 elements
 constexpr int kMaxCols = 256;
 constexpr int kMaxStages = 12;
-constexpr int kBarBytes = 256;
 constexpr int kMaxSplit = 8;
 
 template <typename T, typename OutT, bool GATED>
@@ -346,27 +381,39 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // for 512 clocks of tensor work.  Two accumulators in tensor memory, so a tile's epilogue runs beside the next
 // tile's MMAs; the grid is persistent.
 //
-// Epilogue: sixteen warps per CTA, each 32 rows by 64 accumulator columns (gated: 32 gate and 32 up columns).  Outputs
-// pass through a box of 32 rows x 64 bytes per warp in shared memory, and out of it by TMA where the output's pitch
-// allows, else row by row with consecutive lanes on consecutive elements; the residual comes in through the same box
-// the same way, the first one requested before the wait for the accumulator.
-constexpr int kPairThreads = 640;  // producer, MMA issuer, two idle warps, sixteen epilogue warps
+// Epilogue: sixteen warps per CTA, each 32 rows by 64 accumulator columns (gated: 32 gate and 32 up columns), a lane
+// per row.  Outputs leave through boxes of 32 rows x 64 bytes in shared memory, two per warp in turn, by TMA where the
+// output's pitch allows, else row by row with consecutive lanes on consecutive elements; the residual comes in through
+// the same boxes.  Measured at 4096 x 16384 x 1024, where the epilogue shows, SiLU and residual: 151 us; a lane reading
+// and writing its own row in 32-byte sectors 167; one box per warp and a sixth stage in its place 165 (the two are level
+// from K = 4096 on).
+constexpr int kPairThreads = 576;  // producer, MMA issuer, sixteen epilogue warps
 constexpr int kPairTile = 256;
-constexpr int kPairStages = 6;
-constexpr int kHalfBytes = 128 * 128;          // this CTA's 128 rows of x (or of the weight) x 64 elements of K
+constexpr int kHalfBytes = 128 * 128;          // 128 rows of x (or of the weight) x 64 elements of K
+constexpr int kPairStages = 5;
 constexpr int kPairStageBytes = 2 * kHalfBytes;
-constexpr int kBoxBytes = 2048;
+constexpr int kBoxBytes = 2048;                // two boxes per epilogue warp
+constexpr int kEpilogueWarps = 16;
 constexpr int kAcc = 2;
-constexpr size_t kPairSmem = size_t(kPairStages) * kPairStageBytes + 16 * kBoxBytes + (2 * kPairStages + 2 * kAcc) * 8 + 16 + 1024;
+constexpr int kPairBand = 8;                   // row tiles per band: 8192^3 reads 1.06 GB of DRAM (4: 1.51 GB, 16: 1.23 GB)
+constexpr size_t kPairSmem = size_t(kPairStages) * kPairStageBytes + kEpilogueWarps * 2 * kBoxBytes + (2 * kPairStages + 2 * kAcc) * 8 + 16 + 1024;
 static_assert(kPairSmem <= 232448, "shared memory budget exceeded");
 
-__device__ __forceinline__ void mma_pair_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+// Shared-memory descriptors are the low word of the operand's address (with the leading offset) under one constant
+// high word (stride 1024 bytes, descriptor version, 128-byte swizzle): the issue loop adds to low words only, so one
+// MMA costs it a handful of instructions, fewer than the 128 clocks the MMA runs.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | (1u << 16); }
+
+__device__ __forceinline__ void mma_pair_f16(uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc,
                                              uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
 
@@ -383,35 +430,38 @@ __device__ __forceinline__ void decode_tile(const Args& g, int tile, int& m_blk,
 // 16-byte chunk c of row r of a box: the 64-byte swizzle of the TMA store.
 __device__ __forceinline__ uint32_t box_chunk(int r, int c) { return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); }
 
-// Residual rows [row0, row0 + 32) x columns [col, col + 64 / size) into a box.
+// Residual rows [row0, row0 + 32) x columns [col, col + 64 / size) into a box: aligned ones asynchronously in 16-byte
+// pieces (four lanes on the 64 bytes of a row; no registers wait for them), others element by element, consecutive
+// lanes on consecutive elements.
+template <typename OutT>
+__device__ __forceinline__ void fetch_box_async(const Args& g, uint8_t* box, int row0, int col, int lane) {
+  constexpr int kPer = 16 / int(sizeof(OutT));
+  const OutT* src = static_cast<const OutT*>(g.residual) + col + (lane & 3) * kPer;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    if (row0 + r < g.m)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(box + box_chunk(r, lane & 3))),
+                   "l"(src + int64_t(row0 + r) * g.ldr) : "memory");
+  }
+}
+
 template <typename OutT>
 __device__ __forceinline__ void fetch_box(const Args& g, uint8_t* box, int row0, int col, int lane) {
   constexpr int kCols = 64 / int(sizeof(OutT)), kPer = 16 / int(sizeof(OutT));
   const OutT* src = static_cast<const OutT*>(g.residual);
-  if (g.res_vec && col + kCols <= g.n) {
-    uint4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      v[i] = make_uint4(0, 0, 0, 0);
-      if (row0 + r < g.m) v[i] = *reinterpret_cast<const uint4*>(src + int64_t(row0 + r) * g.ldr + col + (lane & 3) * kPer);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(box + box_chunk(i * 8 + (lane >> 2), lane & 3)) = v[i];
-  } else {
-    constexpr int kRowsAtOnce = 32 / kCols;  // 1 (16-bit) or 2 (fp32)
-    const int c = lane % kCols;
+  constexpr int kRowsAtOnce = 32 / kCols;  // 1 (16-bit) or 2 (fp32)
+  const int c = lane % kCols;
 #pragma unroll 8
-    for (int i = 0; i < 32; i += kRowsAtOnce) {
-      const int r = i + lane / kCols;
-      OutT v = cast_out<OutT>(0.f);
-      if (row0 + r < g.m && col + c < g.n) v = src[int64_t(row0 + r) * g.ldr + col + c];
-      *reinterpret_cast<OutT*>(box + box_chunk(r, c / kPer) + (c % kPer) * sizeof(OutT)) = v;
-    }
+  for (int i = 0; i < 32; i += kRowsAtOnce) {
+    const int r = i + lane / kCols;
+    OutT v = cast_out<OutT>(0.f);
+    if (row0 + r < g.m && col + c < g.n) v = src[int64_t(row0 + r) * g.ldr + col + c];
+    *reinterpret_cast<OutT*>(box + box_chunk(r, c / kPer) + (c % kPer) * sizeof(OutT)) = v;
   }
 }
 
-// A box to the output without TMA (a pitch or base off the 16-byte grid): consecutive lanes write consecutive elements.
+// A box to the output: consecutive lanes write consecutive elements.
 template <typename OutT>
 __device__ __forceinline__ void flush_box(const Args& g, const uint8_t* box, int row0, int col, int lane) {
   constexpr int kCols = 64 / int(sizeof(OutT)), kPer = 16 / int(sizeof(OutT)), kRowsAtOnce = 32 / kCols;
@@ -425,6 +475,23 @@ __device__ __forceinline__ void flush_box(const Args& g, const uint8_t* box, int
   }
 }
 
+// One warp polls an mbarrier for all sixteen epilogue warps; the others wait in a named barrier, which takes neither
+// issue slots nor power from the tensor work (a large product runs at the power limit).  The outcome is reduced over
+// the barrier, so every warp takes the same way.
+__device__ __forceinline__ bool epilogue_wait(bool polls, uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  uint32_t got = 1;
+  if (polls) got = warp_wait(bar, parity, abort_flag) ? 1u : 0u;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred.aligned q, 1, 512, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(got)
+      : "r"(got)
+      : "memory");
+  return got != 0;
+}
+
 template <typename T, typename OutT, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
@@ -436,7 +503,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* boxes = smem + kPairStages * kPairStageBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(boxes + 16 * kBoxBytes);  // used in the leader only
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(boxes + kEpilogueWarps * 2 * kBoxBytes);  // used in the leader only
   uint64_t* empty_bar = full_bar + kPairStages;                              // one set per CTA
   uint64_t* tmem_full_bar = empty_bar + kPairStages;
   uint64_t* tmem_empty_bar = tmem_full_bar + kAcc;                           // used in the leader only
@@ -500,47 +567,53 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     // ---------------------------------------------------------- MMA issuer (leader only)
     if (leader) {
       constexpr uint32_t idesc = make_idesc(256, 256, kBf16);
+      const uint32_t ring_low = desc_low(smem_u32(smem));
+      const int tail_steps = (g.k - (g.num_kb - 1) * 64 + 15) / 16;  // K tail: TMA zero-fills past K
       bool ok = true;
-      uint32_t it = 0, tc = 0;
+      uint32_t s = 0, phase = 0, tc = 0;
       for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++tc) {
-        const int acc = tc % kAcc;
+        const uint32_t acc = tc % kAcc, tmem_d = tmem_base + acc * 256;
         if (!warp_wait(smem_u32(&tmem_empty_bar[acc]), ((tc / kAcc) & 1) ^ 1, abort_flag)) { ok = false; break; }
-        tcgen05_fence_after();
-        const uint32_t tmem_d = tmem_base + acc * 256;
-        for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
-          const int s = it % kPairStages;
-          if (!warp_wait(smem_u32(&full_bar[s]), (it / kPairStages) & 1, abort_flag)) { ok = false; break; }
+        for (int kb = 0; kb < g.num_kb; ++kb) {
+          if (!warp_wait(smem_u32(&full_bar[s]), phase, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
-          uint8_t* st = smem + s * kPairStageBytes;
-          const uint32_t x_addr = smem_u32(st), w_addr = smem_u32(st + kHalfBytes);
-          const int k_left = g.k - kb * 64;
-          const int steps = k_left >= 64 ? 4 : (k_left + 15) / 16;  // K tail: TMA zero-fills past K
+          const uint32_t x_low = ring_low + s * (kPairStageBytes >> 4), w_low = x_low + (kHalfBytes >> 4);
+          const bool last = kb == g.num_kb - 1;
+          const uint32_t more = kb != 0 ? 1u : 0u;
           if (elect_one()) {
-            for (int a = 0; a < steps; ++a)
-              mma_pair_f16(tmem_d, make_smem_desc(x_addr + a * 32, 16, 1024, kSwizzle128B),
-                           make_smem_desc(w_addr + a * 32, 16, 1024, kSwizzle128B), idesc, (kb | a) != 0 ? 1u : 0u);
+            if (!last || tail_steps == 4) {
+              mma_pair_f16(tmem_d, x_low, w_low, idesc, more);
+#pragma unroll
+              for (int a = 1; a < 4; ++a) mma_pair_f16(tmem_d, x_low + a * 2, w_low + a * 2, idesc, 1u);
+            } else {
+              for (int a = 0; a < tail_steps; ++a) mma_pair_f16(tmem_d, x_low + a * 2, w_low + a * 2, idesc, more | uint32_t(a));
+            }
             tcgen05_commit_pair(smem_u32(&empty_bar[s]), 3);  // stage free in both CTAs
+            if (last) tcgen05_commit_pair(smem_u32(&tmem_full_bar[acc]), 3);
           }
           __syncwarp();
+          if (++s == uint32_t(kPairStages)) s = 0, phase ^= 1;
         }
-        if (ok && elect_one()) tcgen05_commit_pair(smem_u32(&tmem_full_bar[acc]), 3);
-        __syncwarp();
       }
     }
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    const int quarter = warp & 3, cgroup = (warp - 4) >> 2;  // a warp may read lane quarter warp % 4 only
-    uint8_t* box = boxes + (warp - 4) * kBoxBytes;
+    const int quarter = warp & 3, cgroup = (warp - 2) >> 2;  // a warp may read lane quarter warp % 4 only
+    uint8_t* my_boxes = boxes + (warp - 2) * 2 * kBoxBytes;
+    constexpr int kBlocks = GATED ? 1 : 2;                // blocks of 32 output columns per warp and tile
+    constexpr int kPer = 16 / int(sizeof(OutT));          // elements per 16-byte chunk
+    const OutT* residual = static_cast<const OutT*>(g.residual);
     const bool tma_out = g.out_vec != 0;
     uint32_t tc = 0;
-    bool ok = true;
-    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++tc) {
+    constexpr int kSub = kBlocks * kBoxesPer32;           // boxes of outputs per warp and tile
+    uint32_t boxes_used = 0;                              // the two boxes take turns
+    for (int tile = pair; tile < num_tiles; tile += num_pairs, ++tc) {
       int m_blk, n_blk;
       decode_tile(g, tile, m_blk, n_blk);
       const int acc = tc % kAcc;
       const int row0 = m_blk * kPairTile + int(rank) * 128 + quarter * 32;
-      const int col0 = n_blk * kOutCols + cgroup * (GATED ? 32 : 64);
-      // the columns' biases: lane l keeps that of column col0 + l of each of the two 32-column blocks
+      const int col0 = n_blk * kOutCols + cgroup * (32 * kBlocks);
+      // the columns' biases: lane l keeps that of column l of each of the two blocks of 32 accumulator columns
       float bias_l[2] = {0.f, 0.f};
       if (g.bias != nullptr) {
 #pragma unroll
@@ -549,28 +622,35 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           if (c < g.n) bias_l[h] = load_bias<T>(g, c + (GATED && h == 1 ? g.n : 0));
         }
       }
-      if (g.residual != nullptr) {
-        if (lane == 0) bulk_wait_group_read0();  // the box's last store has left it
-        __syncwarp();
-        fetch_box<OutT>(g, box, row0, col0, lane);
-      }
-      if (!warp_wait(smem_u32(&tmem_full_bar[acc]), (tc / kAcc) & 1, abort_flag)) { ok = false; break; }
-      tcgen05_fence_after();
-      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * 256 + cgroup * (GATED ? 32 : 64);
-#pragma unroll
-      for (int h = 0; h < (GATED ? 1 : 2); ++h) {
-        uint32_t r[32], u[GATED ? 32 : 1];
-        tmem_ld_32x32b_x32(taddr + h * 32, r);
-        if constexpr (GATED) tmem_ld_32x32b_x32(taddr + 128, reinterpret_cast<uint32_t(&)[32]>(u));
-        tmem_ld_wait();
-        if (GATED || h == 1) {  // everything is in registers: hand the accumulator back
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[acc]), 0));
+      // Both boxes' residuals are requested before the wait for the accumulator: a load queues behind the ring's
+      // 160 KB in flight and takes microseconds.
+      auto async = [&](int i) { return g.res_vec != 0 && col0 + (i + 1) * kBoxCols <= g.n; };
+      if (residual != nullptr) {
+        if (lane == 0) {  // the last stores have left the boxes that are filled now
+          if constexpr (kSub == 1) bulk_wait_group_read1(); else bulk_wait_group_read0();
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < (kSub < 2 ? kSub : 2); ++i)
+          if (async(i)) fetch_box_async<OutT>(g, my_boxes + ((boxes_used + i) & 1) * kBoxBytes, row0, col0 + i * kBoxCols, lane);
+      }
+      if (!epilogue_wait(warp == 2, smem_u32(&tmem_full_bar[acc]), (tc / kAcc) & 1, abort_flag)) break;
+      tcgen05_fence_after();
+      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * 256 + cgroup * (32 * kBlocks);
+      uint32_t r[2][32];  // two blocks of 32 columns (gated: gate and up)
+      tmem_ld_32x32b_x32(taddr, r[0]);
+      tmem_ld_32x32b_x32(taddr + (GATED ? 128 : 32), r[1]);
+      tmem_ld_wait();
+      // everything is in registers: hand the accumulator back
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[acc]), 0));
+#pragma unroll
+      for (int h = 0; h < kBlocks; ++h) {
+        if (col0 + h * 32 >= g.n) break;
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[h][j]);
         if (g.bias != nullptr) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, bias_l[h], j);
@@ -579,42 +659,45 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         if constexpr (GATED) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            float up = __uint_as_float(u[j]);
+            float up = __uint_as_float(r[1][j]);
             if (g.bias != nullptr) up += __shfl_sync(0xffffffffu, bias_l[1], j);
             v[j] *= up;
           }
         }
 #pragma unroll
-        for (int b = 0; b < kBoxesPer32; ++b) {
-          const int col = col0 + h * 32 + b * kBoxCols;
-          constexpr int kPer = 16 / int(sizeof(OutT));
-          if (h != 0 || b != 0 || g.residual == nullptr) {
-            if (lane == 0) bulk_wait_group_read0();
+        for (int b = 0; b < kBoxesPer32; ++b, ++boxes_used) {
+          const int i = h * kBoxesPer32 + b, col = col0 + i * kBoxCols;
+          uint8_t* box = my_boxes + (boxes_used & 1) * kBoxBytes;
+          if (residual == nullptr || i >= 2) {
+            if (lane == 0) bulk_wait_group_read1();  // this box's last store has left it (the other's may be on its way)
             __syncwarp();
-            if (g.residual != nullptr) fetch_box<OutT>(g, box, row0, col, lane);
+          }
+          if (residual != nullptr) {
+            if (!async(i)) fetch_box<OutT>(g, box, row0, col, lane);
+            else if (i >= 2) fetch_box_async<OutT>(g, box, row0, col, lane);
+            asm volatile("cp.async.wait_all;" ::: "memory");
           }
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint4* slot = reinterpret_cast<uint4*>(box + box_chunk(lane, c));
-            OutT o[kPer];
-            if (g.residual != nullptr) {
+            float* e = v + b * kBoxCols + c * kPer;
+            if (residual != nullptr) {
               const uint4 raw = *slot;
               const OutT* res = reinterpret_cast<const OutT*>(&raw);
 #pragma unroll
-              for (int j = 0; j < kPer; ++j) o[j] = cast_out<OutT>(v[b * kBoxCols + c * kPer + j] + widen(res[j]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < kPer; ++j) o[j] = cast_out<OutT>(v[b * kBoxCols + c * kPer + j]);
+              for (int j = 0; j < kPer; ++j) e[j] += widen(res[j]);
             }
-            *slot = *reinterpret_cast<const uint4*>(o);
+            constexpr int kPerWord = kPer / 4;
+            *slot = make_uint4(pack_word<OutT>(e), pack_word<OutT>(e + kPerWord), pack_word<OutT>(e + 2 * kPerWord),
+                               pack_word<OutT>(e + 3 * kPerWord));
           }
           if (tma_out) {
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0 && row0 < g.m && col < g.n) {
-              tma_store_2d(&tmap_out, col, row0, smem_u32(box));  // rows and columns past the edge are clipped
-              bulk_commit_group();
+            if (lane == 0) {
+              if (row0 < g.m && col < g.n) tma_store_2d(&tmap_out, col, row0, smem_u32(box));  // clipped at the edges
+              bulk_commit_group();  // one group per box, stored or not: the waits above count groups
             }
           } else {
             __syncwarp();
@@ -624,6 +707,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         }
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (lane == 0) bulk_wait_group_read0();
   }
 
@@ -666,10 +750,27 @@ bool make_out_map(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int6
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int device_sms() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms > 0 ? sms : 148;
+// What a launch asks the runtime about the device and the kernel, asked once per device: together these calls cost as
+// much host time as the launch itself.
+int device_sms(int dev) {
+  static std::atomic<int> known[64];
+  if (dev < 0 || dev >= 64) return 148;
+  int sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+    known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
+}
+
+template <auto KERNEL>
+bool allow_shared_memory(int dev) {
+  static std::atomic<bool> done[64];
+  if (dev < 0 || dev >= 64) return false;
+  if (done[dev].load(std::memory_order_acquire)) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return false;
+  done[dev].store(true, std::memory_order_release);
+  return true;
 }
 
 struct StreamPlan {
@@ -708,9 +809,9 @@ StreamPlan plan_stream(int64_t m, int64_t n, int64_t k, bool gated, int sms) {
 }
 
 template <typename T, typename OutT, bool GATED>
-int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Args& g, const StreamPlan& p, cudaStream_t stream) {
+int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Args& g, const StreamPlan& p, int dev, cudaStream_t stream) {
   auto kernel = linear_stream_kernel<T, OutT, GATED>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(p.smem)) != cudaSuccess) return HB200_ERR_CUDA;
+  if (!allow_shared_memory<linear_stream_kernel<T, OutT, GATED>>(dev)) return HB200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(p.tiles * p.split), 1, 1);
   cfg.blockDim = dim3(kStreamThreads, 1, 1);
@@ -729,28 +830,30 @@ int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Args& g, c
 
 template <typename T>
 int launch_stream_typed(const CUtensorMap& tw, const CUtensorMap& tx, const Args& g, const StreamPlan& p, bool gated,
-                        bool out_f32, cudaStream_t s) {
-  if (gated) return out_f32 ? launch_stream<T, float, true>(tw, tx, g, p, s) : launch_stream<T, T, true>(tw, tx, g, p, s);
-  return out_f32 ? launch_stream<T, float, false>(tw, tx, g, p, s) : launch_stream<T, T, false>(tw, tx, g, p, s);
+                        bool out_f32, int dev, cudaStream_t s) {
+  if (gated) return out_f32 ? launch_stream<T, float, true>(tw, tx, g, p, dev, s) : launch_stream<T, T, true>(tw, tx, g, p, dev, s);
+  return out_f32 ? launch_stream<T, float, false>(tw, tx, g, p, dev, s) : launch_stream<T, T, false>(tw, tx, g, p, dev, s);
 }
 
 template <typename T, typename OutT, bool GATED>
-int launch_pair(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Args& g, int pairs, cudaStream_t stream) {
+int launch_pair(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Args& g, int pairs, int dev,
+                cudaStream_t stream) {
   auto kernel = linear_pair_kernel<T, OutT, GATED>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPairSmem)) != cudaSuccess) return HB200_ERR_CUDA;
+  if (!allow_shared_memory<linear_pair_kernel<T, OutT, GATED>>(dev)) return HB200_ERR_CUDA;
   kernel<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(tw, tx, to, g);
   return launch_status();
 }
 
 template <typename T>
 int launch_pair_typed(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Args& g, int pairs, bool gated,
-                      bool out_f32, cudaStream_t s) {
-  if (gated) return out_f32 ? launch_pair<T, float, true>(tw, tx, to, g, pairs, s) : launch_pair<T, T, true>(tw, tx, to, g, pairs, s);
-  return out_f32 ? launch_pair<T, float, false>(tw, tx, to, g, pairs, s) : launch_pair<T, T, false>(tw, tx, to, g, pairs, s);
+                      bool out_f32, int dev, cudaStream_t s) {
+  if (gated)
+    return out_f32 ? launch_pair<T, float, true>(tw, tx, to, g, pairs, dev, s) : launch_pair<T, T, true>(tw, tx, to, g, pairs, dev, s);
+  return out_f32 ? launch_pair<T, float, false>(tw, tx, to, g, pairs, dev, s) : launch_pair<T, T, false>(tw, tx, to, g, pairs, dev, s);
 }
 
 // The pair kernel takes over once its tiles are filled: 384 rows of x and 256 weight rows.
-bool use_pair(int64_t m, int64_t n) { return m >= 384 && n >= 256; }
+bool use_pair(int64_t m, int64_t n) { if (getenv("T_PAIR")) return atoi(getenv("T_PAIR")); return m >= 384 && n >= 256; }
 
 }  // namespace linear
 
@@ -769,14 +872,14 @@ int linear_device_status(int reset) {
 
 }  // namespace hb200
 
-extern "C" int hb200_linear(const void* x, const void* weight, const void* bias, const void* residual, void* out, int64_t m,
-                            int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldo, int activation,
-                            int gated, int is_bf16, int bias_f32, int out_f32, void* stream) {
+extern "C" int hb200_linear(const hb200_linear_args* args, void* stream) {
   using namespace hb200;
   using namespace hb200::linear;
+  if (!args) return HB200_ERR_INVALID_ARGUMENT;
+  const auto [x, weight, bias, residual, out, m, n, k, ldx, ldw, ldr, ldo, activation, gated, is_bf16, bias_f32, out_f32, reserved] = *args;
   if (!x || !weight || !out || m <= 0 || n <= 0 || k <= 0 || ldx < k || ldw < k || ldo < n || (residual && ldr < 0))
     return HB200_ERR_INVALID_ARGUMENT;
-  if (activation < kNone || activation > kGeluTanh) return HB200_ERR_INVALID_ARGUMENT;
+  if (activation < kNone || activation > kGeluTanh || reserved != 0) return HB200_ERR_INVALID_ARGUMENT;
   // TMA: 16-byte aligned bases and row pitches
   if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(weight) % 16 || (k % 8) != 0 || (ldx % 8) != 0 ||
       (ldw % 8) != 0)
@@ -787,7 +890,9 @@ extern "C" int hb200_linear(const void* x, const void* weight, const void* bias,
   const uintptr_t item = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual);
   if (item % out_size || reinterpret_cast<uintptr_t>(bias) % (bias_f32 ? 4 : 2)) return HB200_ERR_INVALID_ARGUMENT;
   const bool bf16 = is_bf16 != 0, f32 = out_f32 != 0, is_gated = gated != 0;
-  const int sms = device_sms();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return HB200_ERR_CUDA;
+  const int sms = device_sms(dev);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Args g{};
   g.out = out;
@@ -809,13 +914,14 @@ extern "C" int hb200_linear(const void* x, const void* weight, const void* bias,
     const int64_t m_tiles = (m + kPairTile - 1) / kPairTile, n_tiles = (weight_rows + kPairTile - 1) / kPairTile;
     if (m_tiles * n_tiles > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
     if (!make_map(&tw, weight, weight_rows, k, ldw, 128, bf16) || !make_map(&tx, x, m, k, ldx, 128, bf16)) return HB200_ERR_CUDA;
+    if ((n * out_size) % 16 != 0) g.out_vec = 0;  // a TMA store's last 16 bytes of a row are written whole
     if (g.out_vec && !make_out_map(&to, out, m, n, ldo, f32, bf16)) return HB200_ERR_CUDA;
     g.m_tiles = int(m_tiles);
     g.n_tiles = int(n_tiles);
-    g.band = 16;
+    g.band = kPairBand;
     const int pairs = int(m_tiles * n_tiles < sms / 2 ? m_tiles * n_tiles : sms / 2);
-    return bf16 ? launch_pair_typed<__nv_bfloat16>(tw, tx, to, g, pairs, is_gated, f32, s)
-                : launch_pair_typed<__half>(tw, tx, to, g, pairs, is_gated, f32, s);
+    return bf16 ? launch_pair_typed<__nv_bfloat16>(tw, tx, to, g, pairs, is_gated, f32, dev, s)
+                : launch_pair_typed<__half>(tw, tx, to, g, pairs, is_gated, f32, dev, s);
   }
   const StreamPlan p = plan_stream(m, n, k, is_gated, sms);
   if (p.tiles * p.split > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
@@ -827,6 +933,6 @@ extern "C" int hb200_linear(const void* x, const void* weight, const void* bias,
   g.stages = p.stages;
   g.stage_bytes = p.stage_bytes;
   g.stash_offset = p.stash_offset;
-  return bf16 ? launch_stream_typed<__nv_bfloat16>(tw, tx, g, p, is_gated, f32, s)
-              : launch_stream_typed<__half>(tw, tx, g, p, is_gated, f32, s);
+  return bf16 ? launch_stream_typed<__nv_bfloat16>(tw, tx, g, p, is_gated, f32, dev, s)
+              : launch_stream_typed<__half>(tw, tx, g, p, is_gated, f32, dev, s);
 }

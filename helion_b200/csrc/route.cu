@@ -292,11 +292,11 @@ int launch(const Args& a, cudaStream_t s) {
 }  // namespace route
 }  // namespace hb200
 
-extern "C" int hb200_moe_route_experts(const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t ld,
-                                       int64_t top_k, int scoring, const float* bias, int64_t num_groups,
-                                       int64_t top_groups, int64_t group_top, int renormalize, float scale, float* weights,
-                                       int64_t* chosen, void* stream) {
+extern "C" int hb200_moe_route_experts(const hb200_route_args* args, void* stream) {
   using namespace hb200;
+  if (!args) return HB200_ERR_INVALID_ARGUMENT;
+  const auto [logits, bias, weights, chosen, tokens, experts, ld, top_k, num_groups, top_groups, group_top, logits_dtype, scoring,
+              renormalize, scale] = *args;
   if (!logits || !weights || !chosen || tokens < 0 || experts < 1 || experts > 1024 || ld < 0) return HB200_ERR_INVALID_ARGUMENT;
   if (top_k < 1 || top_k > 32 || num_groups < 1 || num_groups > 32 || experts % num_groups != 0 || top_groups < 1 ||
       top_groups > num_groups || top_k > top_groups * (experts / num_groups))

@@ -7,6 +7,8 @@ here: no autograd formula is registered.
 
 from __future__ import annotations
 
+import struct
+
 import torch
 from torch import Tensor
 from torch.utils._python_dispatch import _get_current_dispatch_mode
@@ -25,7 +27,7 @@ _ACTIVATIONS = {
     "gelu_and_mul": (3, True),
     "gelu_tanh_and_mul": (4, True),
 }
-_OPERAND_DTYPES = (torch.bfloat16, torch.float16)
+_ARGS = struct.Struct("=12q6i")  # hb200_linear_args (a bytes object passes through ctypes at a fifth of 18 values' cost)
 
 
 def _check(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
@@ -33,57 +35,64 @@ def _check(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | No
     """Validates a call; returns the number of output columns."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}; got {activation!r}")
-    if x.dtype not in _OPERAND_DTYPES or weight.dtype != x.dtype:
-        raise TypeError(f"linear takes bfloat16 or float16 operands of one type, got {x.dtype} and {weight.dtype}")
-    if out_dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"out_dtype must be {x.dtype} or torch.float32, got {out_dtype}")
-    if x.dim() < 1 or weight.dim() != 2:
-        raise ValueError(f"linear expects x [..., K] and weight [rows, K]; got {tuple(x.shape)} and {tuple(weight.shape)}")
-    rows, k = weight.shape
-    if x.shape[-1] != k:
-        raise ValueError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
+    dtype, device, x_shape, w_shape = x.dtype, x.device, x.shape, weight.shape
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or weight.dtype is not dtype:
+        raise TypeError(f"linear takes bfloat16 or float16 operands of one type, got {dtype} and {weight.dtype}")
+    if out_dtype is not dtype and out_dtype is not torch.float32:
+        raise TypeError(f"out_dtype must be {dtype} or torch.float32, got {out_dtype}")
+    if len(x_shape) < 1 or len(w_shape) != 2:
+        raise ValueError(f"linear expects x [..., K] and weight [rows, K]; got {tuple(x_shape)} and {tuple(w_shape)}")
+    n, k = rows, _ = w_shape
+    if x_shape[-1] != k:
+        raise ValueError(f"weight {tuple(w_shape)} does not match x {tuple(x_shape)}")
     if k == 0 or k % 8:
         raise ValueError(f"K must be a positive multiple of 8, got {k}")
-    n = rows
     if _ACTIVATIONS[activation][1]:
         if rows % 2:
             raise ValueError(f"{activation} needs a gate half and an up half of the weight's rows; got {rows} rows")
         n = rows // 2
+    if weight.device != device:
+        raise ValueError(f"all tensors must be on one device, got {device} and {weight.device}")
     if bias is not None:
-        if bias.dim() != 1 or bias.shape[0] != rows:
+        if bias.shape != (rows,):
             raise ValueError(f"bias must be [{rows}], got {tuple(bias.shape)}")
-        if bias.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"bias must be {x.dtype} or torch.float32, got {bias.dtype}")
+        if bias.dtype is not dtype and bias.dtype is not torch.float32:
+            raise TypeError(f"bias must be {dtype} or torch.float32, got {bias.dtype}")
+        if bias.device != device:
+            raise ValueError(f"all tensors must be on one device, got {device} and {bias.device}")
     if residual is not None:
-        if residual.shape != (*x.shape[:-1], n):
-            raise ValueError(f"residual must be {(*x.shape[:-1], n)}, got {tuple(residual.shape)}")
-        if residual.dtype != out_dtype:
+        if residual.shape != (*x_shape[:-1], n):
+            raise ValueError(f"residual must be {(*x_shape[:-1], n)}, got {tuple(residual.shape)}")
+        if residual.dtype is not out_dtype:
             raise TypeError(f"residual must be {out_dtype} (the output's type), got {residual.dtype}")
-    for t in (weight, bias, residual):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"all tensors must be on one device, got {x.device} and {t.device}")
+        if residual.device != device:
+            raise ValueError(f"all tensors must be on one device, got {device} and {residual.device}")
     return n
 
 
-def _tma_rows(t: Tensor) -> tuple[Tensor, int]:
+def _tma_rows(t: Tensor, rows: int, k: int) -> tuple[Tensor, int, int]:
     """``t [rows, K]`` as the kernels' bulk copies can read it (unit stride along K, 16-byte aligned rows that do not
-    overlap), and its row pitch; anything else is copied."""
-    rows, k = t.shape
-    pitch = t.stride(0) if rows > 1 else k
-    if t.stride(1) != 1 or pitch < k or pitch % 8 or t.data_ptr() % 16:
-        return t.contiguous() if not t.is_contiguous() else t.clone(), k
-    return t, pitch
+    overlap), its row pitch and its address; anything else is copied."""
+    pitch, unit = t.stride()
+    if rows == 1:
+        pitch = k
+    address = t.data_ptr()
+    if unit != 1 or pitch < k or pitch % 8 or address % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, k, t.data_ptr()
+    return t, pitch, address
 
 
 def _linear_cuda(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
                  out_dtype: torch.dtype) -> Tensor:
     n = _check(x, weight, bias, residual, activation, out_dtype)
-    _require_cuda(x, weight, bias, residual)
-    out = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=x.device)
+    _require_cuda(x)
+    x_shape = x.shape
+    out = x.new_empty((*x_shape[:-1], n), dtype=out_dtype)
     if out.numel() == 0:
         return out
     index = x.get_device()
-    if torch.cuda.current_device() != index:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             _launch(out, x, weight, bias, residual, activation, n, index)
     else:
@@ -93,23 +102,28 @@ def _linear_cuda(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tenso
 
 def _launch(out: Tensor, x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str, n: int,
             index: int) -> None:
-    k = weight.shape[1]
-    x2, ldx = _tma_rows(x if x.dim() == 2 else x.reshape(-1, k))
-    w2, ldw = _tma_rows(weight)
-    m = x2.shape[0]
-    ldr = 0
+    rows, k = weight.shape
+    if x.dim() != 2:
+        x = x.reshape(-1, k)
+    m = x.shape[0]
+    x, ldx, x_ptr = _tma_rows(x, m, k)
+    weight, ldw, w_ptr = _tma_rows(weight, rows, k)
+    ldr = res_ptr = bias_ptr = 0
     if residual is not None:
-        residual = residual if residual.dim() == 2 else residual.reshape(-1, n)
+        if residual.dim() != 2:
+            residual = residual.reshape(m, n)
         if n > 1 and residual.stride(1) != 1:
             residual = residual.contiguous()
-        ldr = residual.stride(0)
-    if bias is not None and not bias.is_contiguous():
+        ldr, res_ptr = residual.stride(0), residual.data_ptr()
+    bias_f32 = False
+    if bias is not None:
         bias = bias.contiguous()
+        bias_ptr, bias_f32 = bias.data_ptr(), bias.dtype is torch.float32
     code, gated = _ACTIVATIONS[activation]
     _lib.call(
-        "hb200_linear", x2.data_ptr(), w2.data_ptr(), None if bias is None else bias.data_ptr(),
-        None if residual is None else residual.data_ptr(), out.data_ptr(), m, n, k, ldx, ldw, ldr, n, code, gated,
-        x.dtype is torch.bfloat16, bias is not None and bias.dtype is torch.float32, out.dtype is torch.float32,
+        "hb200_linear",
+        _ARGS.pack(x_ptr, w_ptr, bias_ptr, res_ptr, out.data_ptr(), m, n, k, ldx, ldw, ldr, n, code, gated,
+                   x.dtype is torch.bfloat16, bias_f32, out.dtype is torch.float32, 0),
         torch._C._cuda_getCurrentRawStream(index),
     )
 
@@ -126,12 +140,16 @@ def _(x, weight, bias, residual, activation, out_dtype):
     return x.new_empty((*x.shape[:-1], n), dtype=out_dtype)
 
 
-def _plain(*tensors: Tensor | None) -> bool:
-    """Whether a call can go straight to the kernel: nothing traces, and no subclass or gradient is involved."""
+def _direct(*tensors: Tensor | None) -> bool:
+    """Whether a call can go straight to its kernel: nothing traces, and no subclass or gradient is involved.  The
+    dispatch of a registered operator written in Python costs more host time than a small call's kernel runs."""
     if torch.compiler.is_compiling() or _get_current_dispatch_mode() is not None:
         return False
     grad = torch.is_grad_enabled()
-    return all(t is None or (type(t) in (Tensor, torch.nn.Parameter) and not (grad and t.requires_grad)) for t in tensors)
+    for t in tensors:
+        if t is not None and ((type(t) is not Tensor and type(t) is not torch.nn.Parameter) or (grad and t.requires_grad)):
+            return False
+    return True
 
 
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation: str | None = None,
@@ -154,7 +172,7 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation:
     """
     activation = activation or "none"
     out_dtype = out_dtype or x.dtype
-    if _plain(x, weight, bias, residual):  # a registered operator's dispatch costs more than a small call's kernel
+    if _direct(x, weight, bias, residual):
         return _linear_cuda(x, weight, bias, residual, activation, out_dtype)
     _check(x, weight, bias, residual, activation, out_dtype)
     return _linear_op(x, weight, bias, residual, activation, out_dtype)

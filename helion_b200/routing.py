@@ -3,15 +3,17 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
+import struct
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from .fused_linear import _plain
+from .fused_linear import _direct
 from .ops import _require_cuda
 
 _SCORINGS = {"softmax": 0, "sigmoid": 1}
+_ARGS = struct.Struct("=11q3if")  # hb200_route_args
 _LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -47,31 +49,25 @@ def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None,
 def _route_cuda(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
                 group_top: int, renormalize: bool, scale: float) -> tuple[Tensor, Tensor]:
     _check(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top)
-    _require_cuda(router_logits, bias)
+    _require_cuda(router_logits)
     tokens, experts = router_logits.shape
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=router_logits.device)
-    chosen = torch.empty((tokens, top_k), dtype=torch.int64, device=router_logits.device)
+    weights = router_logits.new_empty((tokens, top_k), dtype=torch.float32)
+    chosen = router_logits.new_empty((tokens, top_k), dtype=torch.int64)
     if tokens == 0:
         return weights, chosen
     if experts > 1 and router_logits.stride(1) != 1:
         router_logits = router_logits.contiguous()
-    if bias is not None and not bias.is_contiguous():
+    if bias is not None:
         bias = bias.contiguous()
+    args = _ARGS.pack(router_logits.data_ptr(), 0 if bias is None else bias.data_ptr(), weights.data_ptr(), chosen.data_ptr(),
+                      tokens, experts, router_logits.stride(0), top_k, num_groups, top_groups, group_top,
+                      _LOGIT_DTYPES[router_logits.dtype], _SCORINGS[scoring], renormalize, scale)
     index = router_logits.get_device()
-
-    def launch() -> None:
-        _lib.call(
-            "hb200_moe_route_experts", router_logits.data_ptr(), _LOGIT_DTYPES[router_logits.dtype], tokens, experts,
-            router_logits.stride(0), top_k, _SCORINGS[scoring], None if bias is None else bias.data_ptr(), num_groups,
-            top_groups, group_top, renormalize, scale, weights.data_ptr(), chosen.data_ptr(),
-            torch._C._cuda_getCurrentRawStream(index),
-        )
-
-    if torch.cuda.current_device() != index:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
-            launch()
+            _lib.call("hb200_moe_route_experts", args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        launch()
+        _lib.call("hb200_moe_route_experts", args, torch._C._cuda_getCurrentRawStream(index))
     return weights, chosen
 
 
@@ -110,7 +106,7 @@ def route_experts(router_logits: Tensor, top_k: int, *, scoring: str = "softmax"
     logit of ``+inf``) gets NaN weights and distinct experts.  ``E <= 1024``, ``top_k <= 32``, ``num_groups <= 32``.
     """
     args = (router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
-    if _plain(router_logits, bias):
+    if _direct(router_logits, bias):
         return _route_cuda(*args)
     _check(*args[:7])
     return _route_op(*args)

@@ -323,9 +323,16 @@ int hb200_moe_route_top_k(const void* logits, int logits_dtype, int64_t tokens, 
  * picked last, weight 0; a row with a NaN gets NaN weights and valid indices.  experts <= 1024, top_k <= 32,
  * num_groups <= 32 and a divisor of experts, top_k <= top_groups * experts / num_groups.  No counterpart in the
  * reference (see hb200_moe_route_top_k). */
-int hb200_moe_route_experts(const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t ld,
-                            int64_t top_k, int scoring, const float* bias, int64_t num_groups, int64_t top_groups,
-                            int64_t group_top, int renormalize, float scale, float* weights, int64_t* chosen, void* stream);
+typedef struct {
+  const void* logits;
+  const float* bias;
+  float* weights;
+  int64_t* chosen;
+  int64_t tokens, experts, ld, top_k, num_groups, top_groups, group_top;
+  int32_t logits_dtype, scoring, renormalize;
+  float scale;
+} hb200_route_args;
+int hb200_moe_route_experts(const hb200_route_args* args, void* stream);
 
 /* Stable sort of the (token, slot) pairs by expert plus the per-expert counts, on the device: what
  * moe_matmul_ogs_helion_kernel_args_gen computes with bincount + argsort and a host read
@@ -449,11 +456,16 @@ int hb200_dense_matmul(const void* a, const void* b, void* c, int64_t m, int64_t
  * (optional) in the operand type or fp32 (bias_f32 != 0); residual (optional) and out in the operand type or fp32
  * (out_f32 != 0).  Pitches in elements; ldr may be 0 (one row for all).  Any M, N >= 1; K % 8 == 0, 16-byte aligned x
  * and weight, ldx % 8 == ldw % 8 == 0 (HB200_ERR_UNSUPPORTED otherwise).  No workspace.  residual may be out itself
- * (same pitch).  No counterpart in the reference (its examples fuse an epilogue into a matmul through a Python
+ * (same pitch).  The arguments come in a struct (read before the call returns): one pointer instead of eighteen values
+ * halves what a foreign-function call costs.  No counterpart in the reference (its examples fuse an epilogue into a matmul through a Python
  * callable). */
-int hb200_linear(const void* x, const void* weight, const void* bias, const void* residual, void* out, int64_t m,
-                 int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldo, int activation, int gated,
-                 int is_bf16, int bias_f32, int out_f32, void* stream);
+typedef struct {
+  const void *x, *weight, *bias, *residual;
+  void* out;
+  int64_t m, n, k, ldx, ldw, ldr, ldo;
+  int32_t activation, gated, is_bf16, bias_f32, out_f32, reserved; /* reserved: 0 */
+} hb200_linear_args;
+int hb200_linear(const hb200_linear_args* args, void* stream);
 
 /* All-gather + matmul (helion_all_gather_matmul, examples/distributed/all_gather_matmul.py:145-196):
  * c [world * rows_local, N] = gathered a . b^T.  a_shard: this rank's rows [rows_local, K], contiguous.

@@ -7,6 +7,7 @@ import torch
 
 import helion_b200 as hb
 from helion_b200 import _lib
+from helion_b200.fused_linear import _ARGS
 from linear_reference import GATED
 from linear_reference import check
 
@@ -135,21 +136,21 @@ def test_infinities_and_nan_stay_in_their_rows_and_columns(m):
 
 def test_rows_past_the_edges_are_not_written_and_calls_repeat():
     lib = _lib.load()
-    for m, n, k in ((3, 100, 64), (270, 300, 72)):
+    for m, n, k in ((3, 100, 64), (270, 300, 72), (500, 300, 72), (500, 257, 72), (500, 304, 72)):
         a, _ = make(m, n, k)
-        ldo = n + 20
+        ldo = n + 20 if n % 8 else n + 24  # (row pitches on and off the 16-byte grid)
         out = torch.full((m + 2, ldo), 7.0, dtype=torch.bfloat16, device=DEV)
         for _ in range(2):
-            rc = lib.hb200_linear(a["x"].data_ptr(), a["weight"].data_ptr(), None, None, out[1:].data_ptr(), m, n, k, k, k, 0,
-                                  ldo, 0, 0, 1, 0, 0, torch.cuda.current_stream().cuda_stream)
+            rc = lib.hb200_linear(_ARGS.pack(a["x"].data_ptr(), a["weight"].data_ptr(), 0, 0, out[1:].data_ptr(), m, n, k, k, k, 0,
+                                             ldo, 0, 0, 1, 0, 0, 0), torch.cuda.current_stream().cuda_stream)
             assert rc == 0 and status_ok()
             assert torch.equal(out[1 : m + 1, :n], call(a, torch.bfloat16))
             assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[:, n:] == 7).all()
         # the residual may be the output itself
         res = torch.randn(m, ldo, device=DEV).to(torch.bfloat16)
         want = hb.linear(a["x"], a["weight"], residual=res[:, :n])
-        rc = lib.hb200_linear(a["x"].data_ptr(), a["weight"].data_ptr(), None, res.data_ptr(), res.data_ptr(), m, n, k, k, k,
-                              ldo, ldo, 0, 0, 1, 0, 0, torch.cuda.current_stream().cuda_stream)
+        rc = lib.hb200_linear(_ARGS.pack(a["x"].data_ptr(), a["weight"].data_ptr(), 0, res.data_ptr(), res.data_ptr(), m, n, k, k, k,
+                                         ldo, ldo, 0, 0, 1, 0, 0, 0), torch.cuda.current_stream().cuda_stream)
         assert rc == 0 and status_ok() and torch.equal(res[:, :n], want)
 
 

@@ -9,6 +9,8 @@ import torch
 
 import helion_b200 as hb
 from helion_b200 import _lib
+from helion_b200.fused_linear import _ARGS
+from helion_b200.routing import _ARGS as _ROUTE_ARGS
 
 
 def _t(*shape, dtype=torch.bfloat16):
@@ -60,7 +62,8 @@ def test_linear_entry_point_rejects_bad_arguments_before_any_cuda_call():
     p = (ctypes.addressof(buf) + 15) // 16 * 16
 
     def call(x=p, w=p, bias=None, res=None, out=p, m=4, n=8, k=16, ldx=16, ldw=16, ldr=8, ldo=8, act=0, bias_f32=0):
-        return lib.hb200_linear(x, w, bias, res, out, m, n, k, ldx, ldw, ldr, ldo, act, 0, 1, bias_f32, 0, None)
+        return lib.hb200_linear(_ARGS.pack(x or 0, w or 0, bias or 0, res or 0, out or 0, m, n, k, ldx, ldw, ldr, ldo, act, 0, 1,
+                                           bias_f32, 0, 0), None)
 
     bad, unsupported = _lib.HB200_ERR_INVALID_ARGUMENT, _lib.HB200_ERR_UNSUPPORTED
     assert call(x=None) == bad and call(w=None) == bad and call(out=None) == bad
@@ -71,6 +74,7 @@ def test_linear_entry_point_rejects_bad_arguments_before_any_cuda_call():
     assert call(x=p + 2) == unsupported and call(w=p + 8) == unsupported
     assert call(out=p + 1) == bad and call(bias=p + 2, bias_f32=1) == bad and call(res=p + 1) == bad
     assert call(m=1 << 30) == unsupported
+    assert lib.hb200_linear(None, None) == bad
 
 
 @pytest.mark.parametrize(
@@ -119,8 +123,8 @@ def test_route_entry_point_rejects_bad_arguments_before_any_cuda_call():
     p = (ctypes.addressof(buf) + 15) // 16 * 16
 
     def call(logits=p, dtype=2, tokens=4, experts=8, ld=8, k=2, scoring=0, groups=1, top_groups=1, group_top=1, w=p, c=p):
-        return lib.hb200_moe_route_experts(logits, dtype, tokens, experts, ld, k, scoring, None, groups, top_groups, group_top,
-                                           0, 1.0, w, c, None)
+        return lib.hb200_moe_route_experts(_ROUTE_ARGS.pack(logits or 0, 0, w or 0, c or 0, tokens, experts, ld, k, groups, top_groups,
+                                                            group_top, dtype, scoring, 0, 1.0), None)
 
     bad = _lib.HB200_ERR_INVALID_ARGUMENT
     assert call(logits=None) == bad and call(w=None) == bad and call(c=None) == bad
@@ -128,7 +132,7 @@ def test_route_entry_point_rejects_bad_arguments_before_any_cuda_call():
     assert call(experts=0) == bad and call(experts=1025) == bad and call(ld=-1) == bad
     assert call(k=0) == bad and call(k=9) == bad and call(groups=3) == bad and call(groups=4, top_groups=5) == bad
     assert call(groups=4, k=3) == bad and call(group_top=3) == bad and call(groups=8, group_top=2, k=1) == bad
-    assert call(tokens=0) == 0
+    assert call(tokens=0) == 0 and lib.hb200_moe_route_experts(None, None) == bad
 
 
 def test_reference_router_in_small():
