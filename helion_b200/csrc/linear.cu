@@ -7,8 +7,8 @@
 // linear_stream_kernel streams the WEIGHT through the tensor core's M side: a tile is 128 weight rows (64 gate and 64
 // up rows when gated) by up to 256 rows of x, and the accumulator holds y transposed (lane = weight row, column =
 // row of x).  A decode step is bound by the weight's bytes, and one SM streams about 1/148 of the HBM bandwidth, so
-// the K range of a tile is split over a thread-block cluster of 1, 2, 4 or 8 CTAs until there are enough CTAs for the
-// SMs.  The partial sums meet in distributed shared memory: column c of the tile belongs to rank c % split, every
+// the K range of a tile is split over a thread-block cluster of up to 8 CTAs until there are two CTAs for every SM
+// (one, where a tile is wider than 64 rows of x).  The partial sums meet in distributed shared memory: column c of the tile belongs to rank c % split, every
 // rank stores its fp32 partial of a column into the owner's shared memory, and after one cluster barrier the owner
 // adds them in rank order (ascending K: the result does not depend on timing) and runs the epilogue.  No workspace,
 // no counters, no atomics: calls on any streams and replays of any graphs are independent of each other.
@@ -18,7 +18,6 @@
 #include "gemm_common.cuh"
 
 #include <atomic>
-#include <cstdlib>
 #include <type_traits>
 
 namespace hb200 {
@@ -42,11 +41,13 @@ struct Args {
   int out_vec, res_vec;  // 16-byte accesses are possible
   int cols, m_chunks;    // rows of x per tile (a multiple of 16), tiles along M
   int num_kb;            // K blocks of 64 elements
-  int split_log;         // log2 of the CTAs per tile (cluster size)
+  int split;             // stream kernel: CTAs per tile (cluster size)
   int stages, stage_bytes;
   int stash_offset;      // bytes from the ring's start to the partial sums (0: they take the ring's place)
   // pair kernel
   int m_tiles, n_tiles;
+  int split_log;         // log2 of the pairs per tile
+  int tile_cols;         // accumulator columns = weight rows per tile: 128, 192 or 256
   int band;              // row tiles per band of the tile order
 };
 
@@ -185,6 +186,14 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
+// Programmatic dependent launch: the kernel may be resident, its barriers and tensor memory set up, before the kernel
+// in front of it on the stream has finished.  Nothing of global memory, weights included, is touched before that
+// kernel's completion, and the next kernel is let in only after it, so whoever follows sees what a plain order gives.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // The bounded wait as one decision of a converged warp: what follows is executed by all of its lanes or by none.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
@@ -222,11 +231,11 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   const bool overlay = g.stash_offset == 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split_log = g.split_log, split = 1 << split_log, rank = int(cluster_ctarank());
-  const int tile = int(blockIdx.x) >> split_log;
+  const int split = g.split, rank = int(cluster_ctarank());
+  const int tile = int(blockIdx.x) / split;
   const int m0 = (tile % g.m_chunks) * g.cols, n0 = (tile / g.m_chunks) * kOutRows;
   const int kb0 = range_start(rank, g.num_kb, split), kb1 = range_start(rank + 1, g.num_kb, split);
-  const int per = g.cols >> split_log;             // columns this rank owns
+  const int per = (g.cols + split - 1) / split; // columns this rank owns, at most
   const int live_cols = min(g.cols, g.m - m0); // columns past the last row of x are never stored
 
   if (threadIdx.x == 0) {
@@ -250,6 +259,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  wait_for_previous_kernel();
   // A CTA's shared memory may be written by its peers once it runs (or, where the partial sums take the ring's
   // place, once its MMAs have read the ring): arrive here or below, wait in front of the first remote store.
   if (!overlay) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -307,6 +317,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     const int r_in = quarter * 32 + lane;  // weight row inside the tile = accumulator lane
     const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16);
     const uint32_t mine = smem_u32(stash) + uint32_t((rank * per) * 128 + r_in) * 4u;
+    int owner = 0, index = 0;  // of column c: c % split and c / split
 #pragma unroll 1
     for (int c0 = 0; c0 < live_cols; c0 += 8) {
       uint32_t r[8];
@@ -314,8 +325,8 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int c = c0 + j;
-        if (c < live_cols) st_cluster_f32(map_to_cta(mine + uint32_t(c >> split_log) * 512u, uint32_t(c & (split - 1))), __uint_as_float(r[j]));
+        if (c0 + j < live_cols) st_cluster_f32(map_to_cta(mine + uint32_t(index) * 512u, uint32_t(owner)), __uint_as_float(r[j]));
+        if (++owner == split) owner = 0, ++index;
       }
     }
     tcgen05_fence_before();
@@ -328,9 +339,9 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   constexpr int kItemsPerCol = kOutRows / 8;
   for (int item = threadIdx.x; item < per * kItemsPerCol; item += kStreamThreads) {
     const int i = item / kItemsPerCol, piece = (item % kItemsPerCol) * 8;
-    const int row = m0 + (i << split_log) + rank, col = n0 + piece;
+    const int row = m0 + i * split + rank, col = n0 + piece;
     const int valid = g.n - col;
-    if (row >= g.m || valid <= 0) continue;
+    if (i * split + rank >= live_cols || valid <= 0) continue;
     float res[8], acc[8], up[8];
     if (g.residual != nullptr)
       load8(static_cast<const OutT*>(g.residual) + int64_t(row) * g.ldr + col, valid, g.res_vec != 0, res);
@@ -388,15 +399,15 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // and writing its own row in 32-byte sectors 167; one box per warp and a sixth stage in its place 165 (the two are level
 // from K = 4096 on).
 constexpr int kPairThreads = 576;  // producer, MMA issuer, sixteen epilogue warps
-constexpr int kPairTile = 256;
+constexpr int kPairTile = 256;                 // rows of x per tile
 constexpr int kHalfBytes = 128 * 128;          // 128 rows of x (or of the weight) x 64 elements of K
-constexpr int kPairStages = 5;
-constexpr int kPairStageBytes = 2 * kHalfBytes;
+constexpr int kPairRingBytes = 10 * kHalfBytes; // 160 KB: five or six stages
+constexpr int kPairMaxStages = 6;
 constexpr int kBoxBytes = 2048;                // two boxes per epilogue warp
 constexpr int kEpilogueWarps = 16;
 constexpr int kAcc = 2;
 constexpr int kPairBand = 8;                   // row tiles per band: 8192^3 reads 1.06 GB of DRAM (4: 1.51 GB, 16: 1.23 GB)
-constexpr size_t kPairSmem = size_t(kPairStages) * kPairStageBytes + kEpilogueWarps * 2 * kBoxBytes + (2 * kPairStages + 2 * kAcc) * 8 + 16 + 1024;
+constexpr size_t kPairSmem = size_t(kPairRingBytes) + kEpilogueWarps * 2 * kBoxBytes + (2 * kPairMaxStages + 2 * kAcc) * 8 + 16 + 1024;
 static_assert(kPairSmem <= 232448, "shared memory budget exceeded");
 
 // Shared-memory descriptors are the low word of the operand's address (with the leading offset) under one constant
@@ -450,15 +461,18 @@ template <typename OutT>
 __device__ __forceinline__ void fetch_box(const Args& g, uint8_t* box, int row0, int col, int lane) {
   constexpr int kCols = 64 / int(sizeof(OutT)), kPer = 16 / int(sizeof(OutT));
   const OutT* src = static_cast<const OutT*>(g.residual);
-  constexpr int kRowsAtOnce = 32 / kCols;  // 1 (16-bit) or 2 (fp32)
+  constexpr int kRowsAtOnce = 32 / kCols, kLoads = 32 / kRowsAtOnce;  // 32 (16-bit) or 16 (fp32), all in flight at once
   const int c = lane % kCols;
-#pragma unroll 8
-  for (int i = 0; i < 32; i += kRowsAtOnce) {
-    const int r = i + lane / kCols;
-    OutT v = cast_out<OutT>(0.f);
-    if (row0 + r < g.m && col + c < g.n) v = src[int64_t(row0 + r) * g.ldr + col + c];
-    *reinterpret_cast<OutT*>(box + box_chunk(r, c / kPer) + (c % kPer) * sizeof(OutT)) = v;
+  OutT v[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = i * kRowsAtOnce + lane / kCols;
+    v[i] = cast_out<OutT>(0.f);
+    if (row0 + r < g.m && col + c < g.n) v[i] = src[int64_t(row0 + r) * g.ldr + col + c];
   }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+    *reinterpret_cast<OutT*>(box + box_chunk(i * kRowsAtOnce + lane / kCols, c / kPer) + (c % kPer) * sizeof(OutT)) = v[i];
 }
 
 // A box to the output: consecutive lanes write consecutive elements.
@@ -492,32 +506,52 @@ __device__ __forceinline__ bool epilogue_wait(bool polls, uint32_t bar, uint32_t
   return got != 0;
 }
 
-template <typename T, typename OutT, bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__device__ __forceinline__ void st_cluster_v4(uint32_t cluster_addr, const uint32_t (&v)[32], int at) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(v[at]), "r"(v[at + 1]), "r"(v[at + 2]),
+               "r"(v[at + 3]) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive_all() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// SPLIT: fewer tiles than half the pairs of the GPU.  A cluster of two or four pairs works on one tile, each pair on a
+// share of K, and the partial sums meet in distributed shared memory: of the four groups of 64 accumulator columns that
+// a CTA's epilogue warps hold, pair q finishes groups [4 q / split, 4 (q + 1) / split) and receives the others' partials
+// of these, of its own 128 rows, in the place of the ring that all MMAs have read.  They are added in the order of the
+// pairs (own first), so the result does not depend on timing.
+template <typename T, typename OutT, bool GATED, bool SPLIT>
+__global__ void __launch_bounds__(kPairThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                    const __grid_constant__ CUtensorMap tmap_out, const Args g) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kOutCols = GATED ? 128 : 256;           // output columns per tile
+  const int tile_cols = g.tile_cols, out_cols = GATED ? tile_cols / 2 : tile_cols;  // (accumulator, output) columns per tile
+  const int w_bytes = tile_cols * 64;                   // this CTA's half of the tile's weight rows x 64 elements of K
+  const int num_stages = g.stages, stage_bytes = g.stage_bytes;
   constexpr int kBoxCols = 64 / int(sizeof(OutT));      // output columns per box
   constexpr int kBoxesPer32 = 32 / kBoxCols;            // 1 (16-bit outputs) or 2 (fp32)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* boxes = smem + kPairStages * kPairStageBytes;
+  uint8_t* boxes = smem + kPairRingBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(boxes + kEpilogueWarps * 2 * kBoxBytes);  // used in the leader only
-  uint64_t* empty_bar = full_bar + kPairStages;                              // one set per CTA
-  uint64_t* tmem_full_bar = empty_bar + kPairStages;
+  uint64_t* empty_bar = full_bar + kPairMaxStages;                           // one set per CTA
+  uint64_t* tmem_full_bar = empty_bar + kPairMaxStages;
   uint64_t* tmem_empty_bar = tmem_full_bar + kAcc;                           // used in the leader only
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty_bar + kAcc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  const uint32_t cluster_rank = cluster_ctarank(), rank = cluster_rank & 1u;  // rank in the pair
+  const uint32_t leader_rank = cluster_rank & ~1u;
   const bool leader = rank == 0;
-  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const uint16_t pair_mask = uint16_t(3u << leader_rank);
+  const int split_log = SPLIT ? g.split_log : 0, part = SPLIT ? int(cluster_rank >> 1) : 0;
+  // a tile per cluster when split, else tiles dealt to the pairs in turn
+  const int pair = blockIdx.x >> (1 + split_log), num_pairs = gridDim.x >> (1 + split_log);
   const int num_tiles = g.m_tiles * g.n_tiles;
+  const int kb0 = SPLIT ? range_start(part, g.num_kb, 1 << split_log) : 0;
+  const int kb1 = SPLIT ? range_start(part + 1, g.num_kb, 1 << split_log) : g.num_kb;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < num_stages; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);   // the leader's producer arms it; bytes come from both CTAs
       mbar_init(smem_u32(&empty_bar[s]), 1);  // the leader's commit, sent to both CTAs
     }
@@ -539,34 +573,36 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   cluster_sync_all();  // barriers of both CTAs are initialised before anything remote happens
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  wait_for_previous_kernel();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
-    int it = 0;
+    int it = 0, s = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
       int m_blk, n_blk;
       decode_tile(g, tile, m_blk, n_blk);
       const int x_row = m_blk * kPairTile + int(rank) * 128;
-      const int w_row = n_blk * kOutCols + int(rank) * (GATED ? g.n : 128);
-      for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
-        const int s = it % kPairStages;
-        if (!warp_wait(smem_u32(&empty_bar[s]), ((it / kPairStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
-        uint8_t* st = smem + s * kPairStageBytes;
-        const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);  // always the leader's barrier
+      const int w_row = n_blk * out_cols + int(rank) * (GATED ? g.n : tile_cols / 2);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        if (!warp_wait(smem_u32(&empty_bar[s]), phase ^ 1, abort_flag)) { ok = false; break; }
+        uint8_t* st = smem + s * stage_bytes;
+        const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), leader_rank);  // always the leader's barrier
         if (elect_one()) {
-          if (leader) mbar_arrive_expect_tx(smem_u32(&full_bar[s]), 2 * kPairStageBytes);
+          if (leader) mbar_arrive_expect_tx(smem_u32(&full_bar[s]), uint32_t(2 * (kHalfBytes + w_bytes)));
           tma_load_2d_pair(smem_u32(st), &tmap_x, kb * 64, x_row, bar);
           tma_load_2d_pair(smem_u32(st + kHalfBytes), &tmap_w, kb * 64, w_row, bar);
         }
         __syncwarp();
+        if (++s == num_stages) s = 0, phase ^= 1;
       }
     }
-    if (leader && *abort_flag) drain_loads(full_bar, kPairStages, it);
+    if (leader && *abort_flag) drain_loads(full_bar, num_stages, it);
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer (leader only)
     if (leader) {
-      constexpr uint32_t idesc = make_idesc(256, 256, kBf16);
+      const uint32_t idesc = make_idesc(256, tile_cols, kBf16);
       const uint32_t ring_low = desc_low(smem_u32(smem));
       const int tail_steps = (g.k - (g.num_kb - 1) * 64 + 15) / 16;  // K tail: TMA zero-fills past K
       bool ok = true;
@@ -574,25 +610,25 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++tc) {
         const uint32_t acc = tc % kAcc, tmem_d = tmem_base + acc * 256;
         if (!warp_wait(smem_u32(&tmem_empty_bar[acc]), ((tc / kAcc) & 1) ^ 1, abort_flag)) { ok = false; break; }
-        for (int kb = 0; kb < g.num_kb; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!warp_wait(smem_u32(&full_bar[s]), phase, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
-          const uint32_t x_low = ring_low + s * (kPairStageBytes >> 4), w_low = x_low + (kHalfBytes >> 4);
-          const bool last = kb == g.num_kb - 1;
-          const uint32_t more = kb != 0 ? 1u : 0u;
+          const uint32_t x_low = ring_low + s * uint32_t(stage_bytes >> 4), w_low = x_low + (kHalfBytes >> 4);
+          const bool last = kb == kb1 - 1;
+          const uint32_t more = kb != kb0 ? 1u : 0u;
           if (elect_one()) {
-            if (!last || tail_steps == 4) {
+            if (kb != g.num_kb - 1 || tail_steps == 4) {
               mma_pair_f16(tmem_d, x_low, w_low, idesc, more);
 #pragma unroll
               for (int a = 1; a < 4; ++a) mma_pair_f16(tmem_d, x_low + a * 2, w_low + a * 2, idesc, 1u);
             } else {
               for (int a = 0; a < tail_steps; ++a) mma_pair_f16(tmem_d, x_low + a * 2, w_low + a * 2, idesc, more | uint32_t(a));
             }
-            tcgen05_commit_pair(smem_u32(&empty_bar[s]), 3);  // stage free in both CTAs
-            if (last) tcgen05_commit_pair(smem_u32(&tmem_full_bar[acc]), 3);
+            tcgen05_commit_pair(smem_u32(&empty_bar[s]), pair_mask);  // stage free in both CTAs
+            if (last) tcgen05_commit_pair(smem_u32(&tmem_full_bar[acc]), pair_mask);
           }
           __syncwarp();
-          if (++s == uint32_t(kPairStages)) s = 0, phase ^= 1;
+          if (++s == uint32_t(num_stages)) s = 0, phase ^= 1;
         }
       }
     }
@@ -612,10 +648,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       decode_tile(g, tile, m_blk, n_blk);
       const int acc = tc % kAcc;
       const int row0 = m_blk * kPairTile + int(rank) * 128 + quarter * 32;
-      const int col0 = n_blk * kOutCols + cgroup * (32 * kBlocks);
+      const int col0 = n_blk * out_cols + cgroup * (32 * kBlocks);
+      // this warp has columns to finish: the tile is that wide, and (split) they are this pair's
+      const bool mine = cgroup * (32 * kBlocks) < out_cols && (!SPLIT || (cgroup >> (2 - split_log)) == part);
       // the columns' biases: lane l keeps that of column l of each of the two blocks of 32 accumulator columns
       float bias_l[2] = {0.f, 0.f};
-      if (g.bias != nullptr) {
+      if (mine && g.bias != nullptr) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int c = col0 + (GATED ? 0 : h * 32) + lane;
@@ -625,26 +663,65 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       // Both boxes' residuals are requested before the wait for the accumulator: a load queues behind the ring's
       // 160 KB in flight and takes microseconds.
       auto async = [&](int i) { return g.res_vec != 0 && col0 + (i + 1) * kBoxCols <= g.n; };
-      if (residual != nullptr) {
+      if (mine && residual != nullptr) {
         if (lane == 0) {  // the last stores have left the boxes that are filled now
           if constexpr (kSub == 1) bulk_wait_group_read1(); else bulk_wait_group_read0();
         }
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < (kSub < 2 ? kSub : 2); ++i)
-          if (async(i)) fetch_box_async<OutT>(g, my_boxes + ((boxes_used + i) & 1) * kBoxBytes, row0, col0 + i * kBoxCols, lane);
+        for (int i = 0; i < (kSub < 2 ? kSub : 2); ++i) {
+          uint8_t* box = my_boxes + ((boxes_used + i) & 1) * kBoxBytes;
+          if (async(i)) fetch_box_async<OutT>(g, box, row0, col0 + i * kBoxCols, lane);
+          else if (col0 + i * kBoxCols < g.n) fetch_box<OutT>(g, box, row0, col0 + i * kBoxCols, lane);
+        }
       }
-      if (!epilogue_wait(warp == 2, smem_u32(&tmem_full_bar[acc]), (tc / kAcc) & 1, abort_flag)) break;
+      const bool ready = epilogue_wait(warp == 2, smem_u32(&tmem_full_bar[acc]), (tc / kAcc) & 1, abort_flag);
+      if (!SPLIT && !ready) break;  // (split: the cluster's barriers are still to be met)
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * 256 + cgroup * (32 * kBlocks);
       uint32_t r[2][32];  // two blocks of 32 columns (gated: gate and up)
       tmem_ld_32x32b_x32(taddr, r[0]);
-      tmem_ld_32x32b_x32(taddr + (GATED ? 128 : 32), r[1]);
+      tmem_ld_32x32b_x32(taddr + (GATED ? out_cols : 32), r[1]);
       tmem_ld_wait();
       // everything is in registers: hand the accumulator back
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[acc]), 0));
+      if (!SPLIT && lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[acc]), leader_rank));
+      if constexpr (SPLIT) {
+        // groups per pair; slot = [source][group of mine][quarter][block of 32 columns], 4 KB each: 32 lanes x 16 bytes x 8
+        const int own_log = 2 - split_log, owner = cgroup >> own_log, split = 1 << split_log;
+        auto slot = [&](int source) {
+          return uint32_t(((((source << own_log) + (cgroup & ((1 << own_log) - 1))) * 4 + quarter) * 2) * 4096 + lane * 16);
+        };
+        cluster_arrive_all();
+        cluster_wait_all();  // every pair's MMAs have read its ring
+        if (owner != part) {
+          const int index = part < owner ? part : part - 1;  // among the owner's sources
+          const uint32_t dst = map_to_cta(smem_u32(smem) + slot(index), uint32_t(owner * 2) + rank);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) st_cluster_v4(dst + uint32_t(h * 4096 + j * 512), r[h], 4 * j);
+        }
+        __syncwarp();
+        cluster_arrive_all();
+        cluster_wait_all();  // the partial sums are here
+        if (!mine) continue;
+        for (int source = 0; source < split - 1; ++source) {
+          const uint8_t* src = smem + slot(source);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 v = *reinterpret_cast<const float4*>(src + h * 4096 + j * 512);
+              r[h][4 * j] = __float_as_uint(__uint_as_float(r[h][4 * j]) + v.x);
+              r[h][4 * j + 1] = __float_as_uint(__uint_as_float(r[h][4 * j + 1]) + v.y);
+              r[h][4 * j + 2] = __float_as_uint(__uint_as_float(r[h][4 * j + 2]) + v.z);
+              r[h][4 * j + 3] = __float_as_uint(__uint_as_float(r[h][4 * j + 3]) + v.w);
+            }
+        }
+      }
+      if (!mine) continue;
 #pragma unroll
       for (int h = 0; h < kBlocks; ++h) {
         if (col0 + h * 32 >= g.n) break;
@@ -673,8 +750,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             __syncwarp();
           }
           if (residual != nullptr) {
-            if (!async(i)) fetch_box<OutT>(g, box, row0, col, lane);
-            else if (i >= 2) fetch_box_async<OutT>(g, box, row0, col, lane);
+            if (i >= 2 && async(i)) fetch_box_async<OutT>(g, box, row0, col, lane);
+            else if (i >= 2) fetch_box<OutT>(g, box, row0, col, lane);
             asm volatile("cp.async.wait_all;" ::: "memory");
           }
           __syncwarp();
@@ -711,6 +788,15 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     if (lane == 0) bulk_wait_group_read0();
   }
 
+  if constexpr (SPLIT) {
+    if (warp < 2) {  // the two barriers of the exchange
+      __syncwarp();
+      cluster_arrive_all();
+      cluster_wait_all();
+      cluster_arrive_all();
+      cluster_wait_all();
+    }
+  }
   tcgen05_fence_before();
   __syncthreads();
   cluster_sync_all();  // the peer is done with this CTA's shared memory, barriers and tensor memory
@@ -773,16 +859,47 @@ bool allow_shared_memory(int dev) {
   return true;
 }
 
+// How many clusters of `size` CTAs with `smem` bytes each the device holds at once; asked once per device and kind.
+template <auto KERNEL>
+int max_clusters(int dev, int kind, int size, int threads, size_t smem) {
+  static std::atomic<int> known[64][2][4];
+  if (dev < 0 || dev >= 64) return 0;
+  const int log = size == 8 ? 3 : (size == 4 ? 2 : (size == 2 ? 1 : 0));
+  int n = known[dev][kind][log].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(size) * 64, 1, 1);
+    cfg.blockDim = dim3(unsigned(threads), 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(size);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (!allow_shared_memory<KERNEL>(dev) || cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();  // the launch itself will say what is wrong
+      n = -1;
+    }
+    known[dev][kind][log].store(n, std::memory_order_relaxed);
+  }
+  return n > 0 ? n : 0;
+}
+
+constexpr size_t kNarrowSmem = 111 * 1024, kWideSmem = 227 * 1024;
+
 struct StreamPlan {
-  int cols, m_chunks, num_kb, split, split_log, stages, stage_bytes, stash_offset;
+  int cols, m_chunks, num_kb, split, stages, stage_bytes, stash_offset;
   int64_t tiles;
   size_t smem;
 };
 
 // Shared memory decides how many CTAs share an SM, and tensor memory must never run short while they do (a CTA that
 // waits for columns could hold up its cluster peers): narrow tiles (at most 64 columns) get half an SM, wider ones a
-// whole SM.
-StreamPlan plan_stream(int64_t m, int64_t n, int64_t k, bool gated, int sms) {
+// whole SM.  The K range is split while all CTAs run at once and every one keeps four K blocks or more.  One row, 8192 x
+// 28672: 64 tiles over 4 CTAs each 72.8 us, over 2 88.7, over 8 (more CTAs than places) 76.9.
+StreamPlan plan_stream(int64_t m, int64_t n, int64_t k, bool gated, int dev, int sms) {
   StreamPlan p{};
   p.cols = m >= kMaxCols ? kMaxCols : int((m + 15) / 16 * 16);
   p.m_chunks = int((m + p.cols - 1) / p.cols);
@@ -790,22 +907,79 @@ StreamPlan plan_stream(int64_t m, int64_t n, int64_t k, bool gated, int sms) {
   const int out_rows = gated ? 64 : 128;
   p.tiles = ((n + out_rows - 1) / out_rows) * p.m_chunks;
   const bool narrow = p.cols <= 64;
-  const int slots = narrow ? 2 * sms : sms;
+  p.smem = narrow ? kNarrowSmem : kWideSmem;
   p.split = 1;
-  while (p.split < kMaxSplit && p.tiles * p.split * 2 <= slots && p.num_kb >= 8 * p.split) p.split *= 2, ++p.split_log;
+  if (narrow) {
+    const int64_t places = 2 * sms / p.tiles, shares = p.num_kb / 4;
+    const int64_t split = places < shares ? places : shares;
+    p.split = split < 1 ? 1 : (split > kMaxSplit ? kMaxSplit : int(split));
+  } else {
+    while (p.split < kMaxSplit && p.num_kb >= 8 * p.split &&
+           p.tiles <= max_clusters<linear_stream_kernel<__nv_bfloat16, __nv_bfloat16, false>>(dev, 1, p.split * 2, kStreamThreads, p.smem))
+      p.split *= 2;
+  }
   p.stage_bytes = kWBytes + ((p.cols * 128 + 1023) / 1024) * 1024;
-  const int budget = (narrow ? 113 : 227) * 1024 - 2048;  // less barriers and alignment
-  const int stash = p.cols * 512;
-  const int fit_beside = (budget - stash) / p.stage_bytes;
-  const bool beside = narrow;  // wide tiles: the partial sums take the ring's place once it has been read
-  p.stages = beside ? fit_beside : budget / p.stage_bytes;
+  const int budget = int(p.smem) - 2048;  // less barriers and alignment
+  const int stash = (p.cols + p.split - 1) / p.split * p.split * 512;
+  p.stages = (narrow ? budget - stash : budget) / p.stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
-  p.stash_offset = beside ? p.stages * p.stage_bytes : 0;
-  const int body = beside ? p.stages * p.stage_bytes + stash : (p.stages * p.stage_bytes > stash ? p.stages * p.stage_bytes : stash);
-  p.smem = size_t(body) + 2048;
-  const size_t floor = size_t(narrow ? 77 : 116) * 1024;
-  if (p.smem < floor) p.smem = floor;
+  p.stash_offset = narrow ? p.stages * p.stage_bytes : 0;  // wide: the partial sums take the ring's place
   return p;
+}
+
+struct PairPlan {
+  int tile_cols, split_log;
+  int64_t m_tiles, n_tiles;
+};
+
+// Estimated microseconds, from single-GPU measurements of both kernels over N = 1024 .. 28672, K = 1024 .. 28672 and
+// M = 48 .. 2048: they only have to put the forms in the right order (the pick is within 10 % of the best form on that
+// grid, mostly the best).  A pair takes 0.27 us per 64 elements of K and 256 columns, 0.215 for 192 and 0.20 for 128
+// (bound by what an SM gets out of L2, not by the MMAs), a third more when every SM is busy (the clock drops), 7 us for
+// launch, first loads and last epilogue, and 2 to 3 us for an exchange of partial sums.  The stream kernel is bound by
+// the weight's bytes at 5.3 TB/s or by 68 bytes per clock into an SM, and every wave of its CTAs pays for its start and its epilogue.
+PairPlan plan_pair(int64_t m, int64_t weight_rows, int64_t k, int dev, int sms, double* us) {
+  constexpr int kCols[3] = {256, 192, 128};
+  constexpr double kPerBlock[3] = {0.27, 0.215, 0.20}, kExchange[3] = {0.0, 2.0, 3.0};
+  const double num_kb = double((k + 63) / 64);
+  PairPlan best{};
+  *us = 1e30;
+  for (int c = 0; c < 3; ++c) {
+    const int64_t m_tiles = (m + kPairTile - 1) / kPairTile, n_tiles = (weight_rows + kCols[c] - 1) / kCols[c];
+    const int64_t tiles = m_tiles * n_tiles;
+    for (int log = 0; log < 3; ++log) {
+      if (log > 0 && (num_kb < 4 << log ||
+                      tiles > max_clusters<linear_pair_kernel<__nv_bfloat16, __nv_bfloat16, false, true>>(dev, 0, 2 << log, kPairThreads, kPairSmem)))
+        break;
+      const double pairs = sms / 2, busy = double(tiles << log) < pairs ? double(tiles << log) / pairs : 1.0;
+      const double waves = log > 0 ? 1.0 : double((tiles + sms / 2 - 1) / (sms / 2));
+      const double t = 7.0 + kExchange[log] + waves * num_kb / (1 << log) * kPerBlock[c] * (1.0 + 0.35 * busy);
+      if (t < *us) {
+        *us = t;
+        best = PairPlan{kCols[c], log, m_tiles, n_tiles};
+      }
+    }
+  }
+  return best;
+}
+
+double stream_us(const StreamPlan& p, double weight_bytes, int sms) {
+  const double waves = double((p.tiles * p.split + sms - 1) / sms);
+  const double feed = waves * p.num_kb / p.split * (kWBytes + p.cols * 128) / (68.0 * 1900.0);
+  const double memory = weight_bytes / 5.3e6;
+  return 1.1 * (waves * (4.0 + 0.03 * p.cols) + (memory > feed ? memory : feed));
+}
+
+// A cluster of `size` CTAs, launched as a programmatic dependent of whatever precedes it on the stream.
+void launch_attributes(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], unsigned size) {
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
 }
 
 template <typename T, typename OutT, bool GATED>
@@ -817,13 +991,8 @@ int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Args& g, c
   cfg.blockDim = dim3(kStreamThreads, 1, 1);
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(p.split);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  launch_attributes(cfg, attr, unsigned(p.split));
   if (cudaLaunchKernelEx(&cfg, kernel, tw, tx, g) != cudaSuccess) return HB200_ERR_CUDA;
   return HB200_OK;
 }
@@ -835,25 +1004,31 @@ int launch_stream_typed(const CUtensorMap& tw, const CUtensorMap& tx, const Args
   return out_f32 ? launch_stream<T, float, false>(tw, tx, g, p, dev, s) : launch_stream<T, T, false>(tw, tx, g, p, dev, s);
 }
 
-template <typename T, typename OutT, bool GATED>
+template <typename T, typename OutT, bool GATED, bool SPLIT>
 int launch_pair(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Args& g, int pairs, int dev,
                 cudaStream_t stream) {
-  auto kernel = linear_pair_kernel<T, OutT, GATED>;
-  if (!allow_shared_memory<linear_pair_kernel<T, OutT, GATED>>(dev)) return HB200_ERR_CUDA;
-  kernel<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(tw, tx, to, g);
-  return launch_status();
+  auto kernel = linear_pair_kernel<T, OutT, GATED, SPLIT>;
+  if (!allow_shared_memory<linear_pair_kernel<T, OutT, GATED, SPLIT>>(dev)) return HB200_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(2 * pairs), 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  launch_attributes(cfg, attr, SPLIT ? 2u << g.split_log : 2u);
+  if (cudaLaunchKernelEx(&cfg, kernel, tw, tx, to, g) != cudaSuccess) return HB200_ERR_CUDA;
+  return HB200_OK;
 }
 
-template <typename T>
+template <typename T, bool SPLIT>
 int launch_pair_typed(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Args& g, int pairs, bool gated,
                       bool out_f32, int dev, cudaStream_t s) {
   if (gated)
-    return out_f32 ? launch_pair<T, float, true>(tw, tx, to, g, pairs, dev, s) : launch_pair<T, T, true>(tw, tx, to, g, pairs, dev, s);
-  return out_f32 ? launch_pair<T, float, false>(tw, tx, to, g, pairs, dev, s) : launch_pair<T, T, false>(tw, tx, to, g, pairs, dev, s);
+    return out_f32 ? launch_pair<T, float, true, SPLIT>(tw, tx, to, g, pairs, dev, s)
+                   : launch_pair<T, T, true, SPLIT>(tw, tx, to, g, pairs, dev, s);
+  return out_f32 ? launch_pair<T, float, false, SPLIT>(tw, tx, to, g, pairs, dev, s)
+                 : launch_pair<T, T, false, SPLIT>(tw, tx, to, g, pairs, dev, s);
 }
-
-// The pair kernel takes over once its tiles are filled: 384 rows of x and 256 weight rows.
-bool use_pair(int64_t m, int64_t n) { if (getenv("T_PAIR")) return atoi(getenv("T_PAIR")); return m >= 384 && n >= 256; }
 
 }  // namespace linear
 
@@ -910,26 +1085,38 @@ extern "C" int hb200_linear(const hb200_linear_args* args, void* stream) {
   g.num_kb = int((k + 63) / 64);
   const int64_t weight_rows = is_gated ? 2 * n : n;
   CUtensorMap tw, tx, to{};
-  if (use_pair(m, n)) {
-    const int64_t m_tiles = (m + kPairTile - 1) / kPairTile, n_tiles = (weight_rows + kPairTile - 1) / kPairTile;
-    if (m_tiles * n_tiles > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
-    if (!make_map(&tw, weight, weight_rows, k, ldw, 128, bf16) || !make_map(&tx, x, m, k, ldx, 128, bf16)) return HB200_ERR_CUDA;
+  const StreamPlan p = plan_stream(m, n, k, is_gated, dev, sms);
+  double pair_us = 0;
+  // up to 64 rows of x the weight's stream is the work whatever the sizes (6.2 to 6.5 TB/s)
+  const PairPlan q = m > 64 ? plan_pair(m, weight_rows, k, dev, sms, &pair_us) : PairPlan{};
+  if (m > 64 && pair_us < stream_us(p, double(weight_rows) * double(k) * 2, sms)) {
+    if (q.m_tiles * q.n_tiles > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
+    if (!make_map(&tw, weight, weight_rows, k, ldw, q.tile_cols / 2, bf16) || !make_map(&tx, x, m, k, ldx, 128, bf16)) return HB200_ERR_CUDA;
     if ((n * out_size) % 16 != 0) g.out_vec = 0;  // a TMA store's last 16 bytes of a row are written whole
     if (g.out_vec && !make_out_map(&to, out, m, n, ldo, f32, bf16)) return HB200_ERR_CUDA;
-    g.m_tiles = int(m_tiles);
-    g.n_tiles = int(n_tiles);
+    g.m_tiles = int(q.m_tiles);
+    g.n_tiles = int(q.n_tiles);
+    g.tile_cols = q.tile_cols;
     g.band = kPairBand;
-    const int pairs = int(m_tiles * n_tiles < sms / 2 ? m_tiles * n_tiles : sms / 2);
-    return bf16 ? launch_pair_typed<__nv_bfloat16>(tw, tx, to, g, pairs, is_gated, f32, dev, s)
-                : launch_pair_typed<__half>(tw, tx, to, g, pairs, is_gated, f32, dev, s);
+    g.stage_bytes = kHalfBytes + q.tile_cols * 64;
+    g.stages = kPairRingBytes / g.stage_bytes < kPairMaxStages ? kPairRingBytes / g.stage_bytes : kPairMaxStages;
+    g.split_log = q.split_log;
+    const int64_t tiles = q.m_tiles * q.n_tiles;
+    if (q.split_log > 0) {
+      const int pairs = int(tiles << q.split_log);
+      return bf16 ? launch_pair_typed<__nv_bfloat16, true>(tw, tx, to, g, pairs, is_gated, f32, dev, s)
+                  : launch_pair_typed<__half, true>(tw, tx, to, g, pairs, is_gated, f32, dev, s);
+    }
+    const int pairs = int(tiles < sms / 2 ? tiles : sms / 2);
+    return bf16 ? launch_pair_typed<__nv_bfloat16, false>(tw, tx, to, g, pairs, is_gated, f32, dev, s)
+                : launch_pair_typed<__half, false>(tw, tx, to, g, pairs, is_gated, f32, dev, s);
   }
-  const StreamPlan p = plan_stream(m, n, k, is_gated, sms);
   if (p.tiles * p.split > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
   if (!make_map(&tw, weight, weight_rows, k, ldw, is_gated ? 64 : 128, bf16)) return HB200_ERR_CUDA;
   if (!make_map(&tx, x, m, k, ldx, p.cols, bf16)) return HB200_ERR_CUDA;
   g.cols = p.cols;
   g.m_chunks = p.m_chunks;
-  g.split_log = p.split_log;
+  g.split = p.split;
   g.stages = p.stages;
   g.stage_bytes = p.stage_bytes;
   g.stash_offset = p.stash_offset;

@@ -57,6 +57,34 @@ def test_sizes(m, n, k, activation):
     check(y, **a)
 
 
+# sizes at which each form of the CTA-pair kernel runs on 148 SMs: tiles 256, 192 and 128 columns wide, K whole or split
+# over two or four pairs, tiles in one wave and in several
+FORMS = [(2048, 4096, 128), (640, 4096, 2040), (256, 9000, 512), (512, 4096, 4088), (768, 1536, 4096), (256, 4096, 4096),
+         (640, 1024, 4096), (512, 1024, 4088), (512, 512, 4096), (300, 520, 3584), (70, 8200, 1032)]
+
+
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("activation", ["none", "silu_and_mul"])
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_pair_forms(m, n, k, activation, dtype, out):
+    if activation in GATED:
+        n //= 2
+    a, out = make(m, n, k, dtype, activation, dtype, True, out)
+    y = call(a, out)
+    assert status_ok()
+    check(y, **a)
+    assert torch.equal(call(a, out), y)  # partial sums are added in a fixed order
+    # one column fewer than fits any vector or box
+    weight, bias = a["weight"], a["bias"]
+    if activation in GATED:
+        keep = torch.cat([torch.arange(n - 1), n + torch.arange(n - 1)]).to(DEV)
+        weight, bias = weight[keep], bias[keep]
+    else:
+        weight, bias = weight[:-1], bias[:-1]
+    b = dict(a, weight=weight, bias=bias, residual=a["residual"][:, :-1])
+    check(call(b, out), **b)
+
+
 @pytest.mark.parametrize("activation", ACTIVATIONS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,n,k", [(3, 77, 128), (70, 264, 640), (700, 520, 264)])
