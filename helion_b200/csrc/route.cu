@@ -7,15 +7,24 @@
 //   picks:  the top_k best choices of the experts that stay, equal choices by ascending index, masked experts last
 //   weights: the picks' scores (without the bias), divided by their sum if asked for, times scale
 //
-// Which experts come out is decided as in exact arithmetic: choices computed in fp32 are off by less than `margin`
-// (below), and a row in which two neighbouring picks, or the last group that stays and the first that goes, are
-// closer than that is decided again in 64 bits.  Bound by issue and latency, not by bytes.
+// Which experts come out is decided as in exact arithmetic: the fast form orders approximate choices that are off by
+// less than half of `margin` (below), and a row in which two neighbouring picks, or the last group that stays and the
+// first that goes, are closer than that is decided again in 64 bits (choose_exactly).
+//
+// Bound by instructions: at 65536 tokens x 256 experts the bytes take 11 us, and what a warp does per token decides.
+//  * a lane holds VPL neighbouring experts, loaded with one or two vector loads; the bias stays in registers;
+//  * choices become order-preserving 32-bit keys whose last log2(VPL) bits are replaced by the expert's place in the
+//    lane, so the key that wins a lane also says which expert it is (what the bits are worth is in the margin);
+//  * a lane keeps its two best keys; a round takes one redux over the warp, one ballot (the lowest lane wins a tie, as
+//    the lowest index must) and one shuffle, and only a lane that has given up both keys looks through its experts again;
+//  * the picks' logits are read again at the end, by lane r for pick r, instead of travelling through the rounds.
 #include "common.cuh"
 
 namespace hb200 {
 namespace route {
 
 constexpr int kWarps = 8;
+constexpr unsigned kAll = 0xffffffffu;
 
 struct Args {
   const void* logits;
@@ -24,10 +33,13 @@ struct Args {
   float* weights;
   int64_t* chosen;
   int experts, top_k, sigmoid, num_groups, top_groups, group_top, group_size, renormalize;
+  int vec;            // a lane's experts can be read with vector loads
+  int lanes_log;      // log2 of the lanes that look through a group
+  uint32_t group_inv; // ceil(2^20 / group_size): e / group_size = e * group_inv >> 20 for e < 1024
   float scale;
 };
 
-// Order-preserving keys: larger value, larger key; 0 = not to be picked (any more), 1 = masked.  -0 counts as +0.
+// Order-preserving keys: larger value, larger key; -0 counts as +0.
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t u = __float_as_uint(v + 0.f);
   return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
@@ -35,183 +47,85 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
-__device__ __forceinline__ unsigned long long key_of(double v) {
-  const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(v + 0.0));
-  return u ^ (static_cast<unsigned long long>(static_cast<long long>(u) >> 63) | (1ull << 63));
-}
-__device__ __forceinline__ double value_of(unsigned long long k) {
-  return __longlong_as_double(static_cast<long long>((k >> 63) ? k ^ (1ull << 63) : ~k));
-}
-__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(k >> 32));
-  const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(k >> 32) == hi ? uint32_t(k) : 0u);
-  return (static_cast<unsigned long long>(hi) << 32) | lo;
-}
-
-template <typename R> struct KeyOf;
-template <> struct KeyOf<float> { using type = uint32_t; };
-template <> struct KeyOf<double> { using type = unsigned long long; };
-
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-
-template <typename R>
-__device__ __forceinline__ R sigmoid_of(R v) {
-  const R e = exp_of(v < R(0) ? v : -v);
-  return (v < R(0) ? e : R(1)) / (R(1) + e);
-}
+__device__ __forceinline__ float warp_max_of(float v) { return value_of(__reduce_max_sync(kAll, key_of(v))); }
 
 template <typename R>
 __device__ __forceinline__ R warp_total(R v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
+}
+
+// Accurate scores, for weights.
+__device__ __forceinline__ float sigmoid_of(float v) {
+  const float e = expf(-fabsf(v));
+  return (v < 0.f ? e : 1.f) / (1.f + e);
+}
+
+// Scores for choices, from the hardware's exponential and reciprocal.
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// softmax: exp(v - top) / total, otherwise the sigmoid
+__device__ __forceinline__ float score_fast(float v, bool sigmoid, float top, float inv_total) {
+  return sigmoid ? reciprocal_fast(1.f + exp2_fast(-kLog2e * v)) : exp2_fast(kLog2e * (v - top)) * inv_total;
+}
+
+template <typename T, int VPL>
+__device__ __forceinline__ void load_row(const Args& a, const T* row, int lane, float (&l)[VPL]) {
+  if (a.vec) {
+    constexpr int kBytes = VPL * int(sizeof(T)), kWord = kBytes < 16 ? kBytes : 16;
+    T t[VPL];
+    if (lane * VPL < a.experts) {
+#pragma unroll
+      for (int i = 0; i < kBytes / kWord; ++i) {
+        const char* src = reinterpret_cast<const char*>(row + lane * VPL) + i * kWord;
+        char* dst = reinterpret_cast<char*>(t) + i * kWord;
+        if constexpr (kWord == 16) *reinterpret_cast<uint4*>(dst) = __ldg(reinterpret_cast<const uint4*>(src));
+        else if constexpr (kWord == 8) *reinterpret_cast<uint2*>(dst) = __ldg(reinterpret_cast<const uint2*>(src));
+        else if constexpr (kWord == 4) *reinterpret_cast<uint32_t*>(dst) = __ldg(reinterpret_cast<const uint32_t*>(src));
+        else *reinterpret_cast<uint16_t*>(dst) = __ldg(reinterpret_cast<const uint16_t*>(src));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) l[j] = lane * VPL < a.experts ? float(t[j]) : -INFINITY;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) l[j] = lane * VPL + j < a.experts ? float(row[lane * VPL + j]) : -INFINITY;
+  }
 }
 
 struct Picks {
   int expert;   // lane r holds pick r
   float logit;
-  bool unsure;  // two values that decide the result are closer than the arithmetic can tell
 };
 
-template <typename T, int VPL>
-__device__ __forceinline__ void load_row(const Args& a, int64_t token, int lane, float (&l)[VPL], float (&b)[VPL]) {
-  const T* row = static_cast<const T*>(a.logits) + token * a.ld;
+// ------------------------------------------------------------------ exact form, for the few rows that need it
+__device__ __forceinline__ double warp_best(double v) {
 #pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    const int e = lane * VPL + j;
-    l[j] = e < a.experts ? float(row[e]) : -INFINITY;
-    b[j] = (a.bias != nullptr && e < a.experts) ? a.bias[e] : 0.f;
+  for (int o = 16; o > 0; o >>= 1) {
+    const double other = __shfl_xor_sync(kAll, v, o);
+    v = other > v ? other : v;
   }
-}
-
-// top, total: the row's largest logit and sum of exp(logit - top) (softmax only)
-template <typename R, int VPL>
-__device__ __forceinline__ Picks choose(const Args& a, int lane, const float (&l)[VPL], const float (&b)[VPL], float top, R total) {
-  using Key = typename KeyOf<R>::type;
-  constexpr bool kExact = sizeof(R) == 8;
-  constexpr unsigned kAll = 0xffffffffu;
-  const bool biased = a.bias != nullptr;
-  // fp32 scores are off by at most 5 units of 2^-24 (sigmoid: one exponential, one addition, one division of values
-  // up to 1) or 17 (softmax: rounding of logit - top scaled by score, the sum's own error); the sum with the bias
-  // adds half a unit in the last place of the choice.  Twice that separates two choices, rounded up.
-  const R base = a.sigmoid ? R(1.0 / (1 << 20)) : R(1.0 / (1 << 18));
-  auto margin = [&](R v) { return base + (v < R(0) ? -v : v) * R(1.0 / (1 << 22)); };
-  auto score = [&](float logit) -> R {
-    return a.sigmoid ? sigmoid_of(R(logit)) : exp_of(R(logit) - R(top)) / total;
-  };
-
-  Key key[VPL];
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    const int e = lane * VPL + j;
-    const bool live = l[j] > -INFINITY;
-    R choice = R(l[j]);
-    if (biased) choice = (live ? score(l[j]) : R(0)) + R(b[j]);
-    key[j] = e >= a.experts ? Key(0) : (live && choice > R(-INFINITY)) ? key_of(choice) : Key(1);
-  }
-  bool unsure = false;
-
-  if (a.num_groups > 1) {
-    R mine = R(-INFINITY);
-    for (int g = 0; g < a.num_groups; ++g) {
-      const int lo = g * a.group_size, hi = lo + a.group_size;
-      Key m1 = 0, m2 = 0;
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const int e = lane * VPL + j;
-        if (e >= lo && e < hi) {
-          if (key[j] > m1) { m2 = m1; m1 = key[j]; } else if (key[j] > m2) { m2 = key[j]; }
-        }
-      }
-      const Key best = warp_max(m1);
-      R s = R(-INFINITY);
-      if (best > Key(1)) {
-        const bool of_scores = a.group_top > 1 && !biased;
-        s = of_scores ? score(float(value_of(best))) : R(value_of(best));
-        if (a.group_top > 1) {
-          const int at = __ffs(__ballot_sync(kAll, m1 == best)) - 1;
-          const Key next = warp_max(lane == at ? m2 : m1);
-          if (next > Key(1)) s += of_scores ? score(float(value_of(next))) : R(value_of(next));
-        }
-      }
-      if (lane == g) mine = s;
-    }
-    int before = 0;
-    for (int g = 0; g < a.num_groups; ++g) {
-      const R other = __shfl_sync(kAll, mine, g);
-      before += other > mine || (other == mine && g < lane);
-    }
-    const bool stays = lane < a.num_groups && before < a.top_groups;
-    const unsigned kept = __ballot_sync(kAll, stays);
-    if (!kExact && (biased || a.group_top > 1) && a.top_groups < a.num_groups) {
-      const Key last = ~warp_max(stays ? Key(~key_of(mine)) : Key(0));
-      const Key first = warp_max(lane < a.num_groups && !stays ? key_of(mine) : Key(0));
-      const R lv = R(value_of(last)), fv = R(value_of(first));
-      if (fv > R(-INFINITY) && lv - fv <= R(2) * margin(lv)) unsure = true;
-    }
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-      const int e = lane * VPL + j;
-      if (e < a.experts && !((kept >> (e / a.group_size)) & 1u)) key[j] = 0;
-    }
-  }
-
-  Picks p{0, -INFINITY, false};
-  Key prev = 0;
-  float prev_l = 0.f, prev_b = 0.f;
-  const int rounds = a.top_k + (!kExact && biased ? 1 : 0);  // one more to compare the last pick with what it left behind
-  for (int r = 0; r < rounds; ++r) {
-    Key m = 0;
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) m = key[j] > m ? key[j] : m;
-    const Key best = warp_max(m);
-    const int at = __ffs(__ballot_sync(kAll, m == best)) - 1;
-    int e = 0;
-    float pl = 0.f, pb = 0.f;
-    if (lane == at) {
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        if (!found && key[j] == best) {
-          found = true;
-          key[j] = 0;
-          e = lane * VPL + j;
-          pl = l[j];
-          pb = b[j];
-        }
-      }
-    }
-    e = __shfl_sync(kAll, e, at);
-    pl = __shfl_sync(kAll, pl, at);
-    if (!kExact && biased) {
-      pb = __shfl_sync(kAll, pb, at);
-      if (r > 0 && best > Key(1)) {
-        const R hi = R(value_of(prev)), lo = R(value_of(best));
-        if (hi - lo <= margin(hi) && !(pl == prev_l && pb == prev_b)) unsure = true;
-      }
-      prev = best;
-      prev_l = pl;
-      prev_b = pb;
-    }
-    if (lane == r && r < a.top_k) {
-      p.expert = e;
-      p.logit = pl;
-    }
-  }
-  p.unsure = unsure;
-  return p;
+  return v;
 }
 
 template <typename T, int VPL>
-__device__ __noinline__ Picks choose_exactly(const Args& a, int64_t token, int lane) {
-  float l[VPL], b[VPL];
-  load_row<T, VPL>(a, token, lane, l, b);
+__device__ __noinline__ Picks choose_exactly(const Args& a, const T* row, int lane) {
+  float l[VPL];
+  load_row<T, VPL>(a, row, lane, l);
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < VPL; ++j) top = fmaxf(top, l[j]);
-  top = hb200::warp_max(top);
+  top = warp_max_of(top);
   double total = 0.0;
   if (!a.sigmoid) {
 #pragma unroll
@@ -219,52 +133,256 @@ __device__ __noinline__ Picks choose_exactly(const Args& a, int64_t token, int l
       if (l[j] > -INFINITY) total += exp(double(l[j]) - double(top));
     total = warp_total(total);
   }
-  return choose<double, VPL>(a, lane, l, b, top, total);
-}
-
-template <typename T, int VPL>
-__global__ void __launch_bounds__(kWarps * 32)
-route_experts_kernel(const __grid_constant__ Args a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t step = int64_t(gridDim.x) * kWarps;
-  for (int64_t token = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); token < a.tokens; token += step) {
-    float l[VPL], b[VPL];
-    load_row<T, VPL>(a, token, lane, l, b);
-    // A NaN (or, under softmax, an infinite logit) spoils the row's scores: its weights come out as NaN.
-    bool spoilt = false;
-    float top = -INFINITY;
+  auto score = [&](double v) {
+    if (!a.sigmoid) return exp(v - double(top)) / total;
+    const double e = exp(v < 0.0 ? v : -v);
+    return (v < 0.0 ? e : 1.0) / (1.0 + e);
+  };
+  // rank: 2 live, 1 masked, 0 not to be picked (any more); within a rank the choice decides (masked: the index alone)
+  double choice[VPL];
+  uint32_t live = 0, open = 0;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    const int e = lane * VPL + j;
+    choice[j] = double(l[j]);
+    if (a.bias != nullptr && e < a.experts && l[j] > -INFINITY) choice[j] = score(double(l[j])) + double(a.bias[e]);
+    if (e < a.experts) open |= 1u << j;
+    if (e < a.experts && l[j] > -INFINITY && choice[j] > -INFINITY) live |= 1u << j;
+  }
+  if (a.num_groups > 1) {
+    const bool of_scores = a.group_top > 1 && a.bias == nullptr;
+    double mine = -INFINITY;
+    for (int g = 0; g < a.num_groups; ++g) {
+      const int lo = g * a.group_size, hi = lo + a.group_size;
+      double s = -INFINITY;
+      uint32_t left = live;
+      for (int i = 0; i < a.group_top; ++i) {
+        double m = -INFINITY;
+        int at_j = -1;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+          const int e = lane * VPL + j;
+          if (e >= lo && e < hi && ((left >> j) & 1u) && (at_j < 0 || choice[j] > m)) m = choice[j], at_j = j;
+        }
+        const unsigned some = __ballot_sync(kAll, at_j >= 0);
+        if (some == 0) break;
+        const double best = warp_best(m);
+        const int at = __ffs(__ballot_sync(kAll, at_j >= 0 && m == best)) - 1;
+        if (lane == at) left &= ~(1u << at_j);
+        const double value = of_scores ? score(best) : best;
+        s = i == 0 ? value : s + value;
+      }
+      if (lane == g) mine = s;
+    }
+    int before = 0;
+    for (int g = 0; g < a.num_groups; ++g) {
+      const double other = __shfl_sync(kAll, mine, g);
+      before += other > mine || (other == mine && g < lane);
+    }
+    const unsigned kept = __ballot_sync(kAll, lane < a.num_groups && before < a.top_groups);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if ((open >> j) & 1u && !((kept >> ((lane * VPL + j) / a.group_size)) & 1u)) open &= ~(1u << j);
+  }
+  Picks p{0, -INFINITY};
+  for (int r = 0; r < a.top_k; ++r) {
+    int rank = 0, at_j = 0;
+    double m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-      spoilt |= l[j] != l[j] || b[j] != b[j] || (!a.sigmoid && l[j] == INFINITY);
-      top = fmaxf(top, l[j]);
+      if (!((open >> j) & 1u)) continue;
+      const int mine = 1 + int((live >> j) & 1u);
+      if (mine > rank || (mine == rank && mine == 2 && choice[j] > m)) rank = mine, m = choice[j], at_j = j;
     }
-    spoilt = __any_sync(0xffffffffu, spoilt);
-    top = hb200::warp_max(top);
-    float total = 0.f;
-    if (!a.sigmoid) {
+    const int best_rank = __reduce_max_sync(kAll, rank);
+    const double best = warp_best(rank == best_rank && rank == 2 ? m : -INFINITY);
+    const int at = __ffs(__ballot_sync(kAll, rank == best_rank && (rank < 2 || m == best))) - 1;
+    float logit = 0.f;
 #pragma unroll
-      for (int j = 0; j < VPL; ++j)
-        if (l[j] > -INFINITY) total += expf(l[j] - top);
+    for (int j = 0; j < VPL; ++j)
+      if (j == at_j) logit = l[j];
+    if (lane == at) open &= ~(1u << at_j);
+    const int e = __shfl_sync(kAll, lane * VPL + at_j, at);
+    logit = __shfl_sync(kAll, logit, at);
+    if (lane == r) p.expert = e, p.logit = logit;
+  }
+  return p;
+}
+
+// ------------------------------------------------------------------ fast form
+constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
+
+// (the exact form, a call that few rows make, would otherwise set the registers and with them the occupancy)
+template <typename T, int VPL, bool GROUPS>
+__global__ void __launch_bounds__(kWarps * 32, VPL <= 8 ? 4 : (VPL == 16 ? 2 : 1))
+route_experts_kernel(const __grid_constant__ Args a) {
+  constexpr uint32_t kPlace = VPL - 1;  // the key bits that hold an expert's place in its lane, counted down
+  constexpr uint32_t kMasked = VPL;     // key of a masked expert: below every live one, above 0 (not to be picked)
+  __shared__ uint32_t shared_keys[GROUPS ? kWarps : 1][GROUPS ? 32 * VPL : 1];
+  uint32_t* group_keys = shared_keys[GROUPS ? threadIdx.x >> 5 : 0];
+  const int lane = threadIdx.x & 31;
+  const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr;
+  const bool by_scores = GROUPS && a.group_top > 1;  // group scores are sums of scores
+  // Half of a margin is what one choice may be off by.  Sigmoid: 7 units of 2^-24 (its argument's rounding, one
+  // exponential, one addition, one reciprocal, of values up to 1); softmax: up to 30 (the rounding of logit - top
+  // scaled by the score, the sum's own error); the bias's addition half a unit in the last place; and the place bits
+  // cut VPL units off the key.  Without a bias the logits themselves are compared.
+  const float base = !biased ? 1e-36f : (sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18));
+  auto margin = [&](float v) { return base + fabsf(v) * ((VPL + 2) * (1.f / (1 << 23))); };
+
+  float b[VPL];
+  bool bias_spoilt = false;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    b[j] = (biased && lane * VPL + j < a.experts) ? a.bias[lane * VPL + j] : 0.f;
+    bias_spoilt |= b[j] != b[j];
+  }
+
+  const int64_t step = int64_t(gridDim.x) * kWarps;
+  for (int64_t token = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); token < a.tokens; token += step) {
+    const T* row = static_cast<const T*>(a.logits) + token * a.ld;
+    float l[VPL];
+    load_row<T, VPL>(a, row, lane, l);
+    // A NaN (or, under softmax, an infinite logit) spoils the row's scores: its weights come out as NaN.
+    bool spoilt = bias_spoilt;
+    float top = -INFINITY, total = 0.f, inv_total = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) spoilt |= l[j] != l[j] || (!sigmoid && l[j] == INFINITY);
+    spoilt = __any_sync(kAll, spoilt);
+    if (!sigmoid && (biased || by_scores || !a.renormalize)) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) top = fmaxf(top, l[j]);
+      top = warp_max_of(top);
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) total += l[j] > -INFINITY ? exp2_fast(kLog2e * (l[j] - top)) : 0.f;
       total = warp_total(total);
+      inv_total = reciprocal_fast(total);
     }
-    Picks p = choose<float, VPL>(a, lane, l, b, top, total);
-    if (p.unsure && !spoilt) p = choose_exactly<T, VPL>(a, token, lane);
+
+    uint32_t key[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const bool live = l[j] > -INFINITY;
+      float choice = l[j];
+      if (biased) choice = live ? score_fast(l[j], sigmoid, top, inv_total) + b[j] : -INFINITY;
+      key[j] = choice > -INFINITY ? key_of(choice) : kMasked;  // (a NaN is masked)
+      if (lane * VPL + j >= a.experts) key[j] = 0;
+    }
+    bool unsure = false;
+
+    if constexpr (GROUPS) {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) group_keys[lane * VPL + j] = key[j];
+      __syncwarp();
+      // 2^lanes_log lanes look through a group
+      const int lanes = 1 << a.lanes_log, group = lane >> a.lanes_log;
+      uint32_t m1 = 0, m2 = 0;
+      if (group < a.num_groups) {
+        for (int i = lane & (lanes - 1); i < a.group_size; i += lanes) {
+          const uint32_t k = group_keys[group * a.group_size + i];
+          m2 = max(m2, min(m1, k));
+          m1 = max(m1, k);
+        }
+      }
+      for (int o = 1; o < lanes; o <<= 1) {
+        const uint32_t o1 = __shfl_xor_sync(kAll, m1, o), o2 = __shfl_xor_sync(kAll, m2, o);
+        m2 = max(max(m2, o2), min(m1, o1));
+        m1 = max(m1, o1);
+      }
+      float s = -INFINITY;
+      if (m1 > kMasked) {
+        const bool convert = by_scores && !biased;
+        s = convert ? score_fast(value_of(m1), sigmoid, top, inv_total) : value_of(m1);
+        if (by_scores && m2 > kMasked) s += convert ? score_fast(value_of(m2), sigmoid, top, inv_total) : value_of(m2);
+      }
+      int before = 0;
+      for (int g = 0; g < a.num_groups; ++g) {
+        const float other = __shfl_sync(kAll, s, g << a.lanes_log);
+        before += other > s || (other == s && g < group);
+      }
+      const bool is_group = group < a.num_groups, stays = is_group && before < a.top_groups;
+      const unsigned kept = __ballot_sync(kAll, stays);
+      if (a.top_groups < a.num_groups) {
+        const float last = value_of(~__reduce_max_sync(kAll, stays ? ~key_of(s) : 0u));
+        const float first = value_of(__reduce_max_sync(kAll, is_group && !stays ? key_of(s) : 0u));
+        // sums of two are off by twice as much, and scores of logits by a softmax's margin at most
+        const float slack = by_scores ? 2.f * margin(last) + (biased ? 0.f : 1.f / (1 << 17)) : (biased ? margin(last) : 0.f);
+        unsure = first > -INFINITY && last - first <= slack && slack > 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const uint32_t g = (uint32_t(lane * VPL + j) * a.group_inv) >> 20;
+        if (!((kept >> ((g << a.lanes_log) & 31u)) & 1u)) key[j] = 0;
+      }
+    }
+
+    // a lane's two best keys, the experts' places in their last bits
+    uint32_t m1 = 0, m2 = 0;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      if (key[j] != 0) key[j] = (key[j] & ~kPlace) | (kPlace - j);
+      m2 = max(m2, min(m1, key[j]));
+      m1 = max(m1, key[j]);
+    }
+    bool have2 = true;
+    uint32_t pick_key = 0, left_key = 0;
+    int pick_lane = 0, left_lane = 0;
+    for (int r = 0; r <= a.top_k; ++r) {  // one more, to compare the last pick with what it left behind
+      const uint32_t mine = m1 & ~kPlace, best = __reduce_max_sync(kAll, mine);
+      const int at = __ffs(__ballot_sync(kAll, mine == best)) - 1;
+      const uint32_t won = __shfl_sync(kAll, m1, at);
+      if (lane == r) pick_key = won, pick_lane = at;
+      left_key = won, left_lane = at;
+      if (lane == at) {
+        if (have2) {
+          m1 = m2;
+          have2 = false;
+        } else {
+          m1 = 0;
+#pragma unroll
+          for (int j = 0; j < VPL; ++j) m1 = key[j] < won ? max(m1, key[j]) : m1;
+        }
+      }
+    }
+    auto expert_of = [&](uint32_t k, int at) { return at * VPL + int(kPlace - (k & kPlace)); };
+    Picks p{expert_of(pick_key, pick_lane), -INFINITY};
+    if (lane < a.top_k) p.logit = float(row[p.expert]);
+    {
+      uint32_t next_key = __shfl_down_sync(kAll, pick_key, 1);
+      if (lane == a.top_k - 1) next_key = left_key;
+      const float hi = value_of(pick_key & ~kPlace), lo = value_of(next_key & ~kPlace);
+      bool close = lane < a.top_k && (next_key & ~kPlace) > kMasked && hi - lo <= margin(hi);
+      if (__any_sync(kAll, close)) {  // equal inputs are a tie whatever the precision
+        const int left = min(expert_of(left_key, left_lane), a.experts - 1);
+        float next_logit = __shfl_down_sync(kAll, p.logit, 1), next_bias = 0.f, bias = 0.f;
+        if (lane == a.top_k - 1) next_logit = float(row[left]);
+        if (biased) {
+          bias = a.bias[min(p.expert, a.experts - 1)];
+          next_bias = __shfl_down_sync(kAll, bias, 1);
+          if (lane == a.top_k - 1) next_bias = a.bias[left];
+        }
+        close = close && !(p.logit == next_logit && bias == next_bias);
+      }
+      unsure = __any_sync(kAll, unsure || close);
+    }
+    if (unsure && !spoilt) p = choose_exactly<T, VPL>(a, row, lane);
 
     // Weights.  Renormalised ones are ratios of scores: they are formed relative to the largest pick, so that picks
     // far below the row's largest logit (a bias or a group can choose them) keep their ratios.
     const bool live = lane < a.top_k && p.logit > -INFINITY;
     float w = 0.f;
     if (a.renormalize) {
-      const float best = hb200::warp_max(live ? p.logit : -INFINITY);
+      const float best = warp_max_of(live ? p.logit : -INFINITY);
       if (live) {
-        if (!a.sigmoid) w = expf(p.logit - best);
+        if (!sigmoid) w = expf(p.logit - best);
         else if (p.logit >= 0.f) w = 1.f / (1.f + expf(-p.logit));
         else w = expf(p.logit - fminf(best, 0.f)) / (1.f + expf(p.logit));
       }
       const float sum = warp_total(w);
       if (live) w = w / sum;
     } else if (live) {
-      w = a.sigmoid ? sigmoid_of(p.logit) : expf(p.logit - top) / total;
+      w = sigmoid ? sigmoid_of(p.logit) : expf(p.logit - top) / total;
     }
     w = spoilt ? NAN : w * a.scale;
     if (lane < a.top_k) {
@@ -274,19 +392,25 @@ route_experts_kernel(const __grid_constant__ Args a) {
   }
 }
 
-template <typename T>
-int launch(const Args& a, cudaStream_t s) {
+template <typename T, int VPL>
+int launch_vpl(Args& a, cudaStream_t s) {
+  constexpr int kBytes = VPL * int(sizeof(T)), kWord = kBytes < 16 ? kBytes : 16;
+  a.vec = a.experts % VPL == 0 && reinterpret_cast<uintptr_t>(a.logits) % kWord == 0 && (a.ld * int64_t(sizeof(T))) % kWord == 0;
   const int64_t blocks = (a.tokens + kWarps - 1) / kWarps;
-  const int grid = int(blocks < 148 * 8 ? blocks : 148 * 8);
-#define HB200_ROUTE(V) route_experts_kernel<T, V><<<grid, kWarps * 32, 0, s>>>(a)
-  if (a.experts <= 32) HB200_ROUTE(1);
-  else if (a.experts <= 64) HB200_ROUTE(2);
-  else if (a.experts <= 128) HB200_ROUTE(4);
-  else if (a.experts <= 256) HB200_ROUTE(8);
-  else if (a.experts <= 512) HB200_ROUTE(16);
-  else HB200_ROUTE(32);
-#undef HB200_ROUTE
+  const int grid = int(blocks < 148 * 16 ? blocks : 148 * 16);
+  if (a.num_groups > 1) route_experts_kernel<T, VPL, true><<<grid, kWarps * 32, 0, s>>>(a);
+  else route_experts_kernel<T, VPL, false><<<grid, kWarps * 32, 0, s>>>(a);
   return launch_status();
+}
+
+template <typename T>
+int launch(Args& a, cudaStream_t s) {
+  if (a.experts <= 32) return launch_vpl<T, 1>(a, s);
+  if (a.experts <= 64) return launch_vpl<T, 2>(a, s);
+  if (a.experts <= 128) return launch_vpl<T, 4>(a, s);
+  if (a.experts <= 256) return launch_vpl<T, 8>(a, s);
+  if (a.experts <= 512) return launch_vpl<T, 16>(a, s);
+  return launch_vpl<T, 32>(a, s);
 }
 
 }  // namespace route
@@ -320,6 +444,9 @@ extern "C" int hb200_moe_route_experts(const hb200_route_args* args, void* strea
   a.group_size = int(experts / num_groups);
   a.renormalize = renormalize != 0;
   a.scale = scale;
+  a.lanes_log = 0;
+  while ((num_groups << (a.lanes_log + 1)) <= 32) ++a.lanes_log;
+  a.group_inv = uint32_t(((1 << 20) + a.group_size - 1) / a.group_size);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (logits_dtype == 0) return route::launch<__nv_bfloat16>(a, s);
   if (logits_dtype == 1) return route::launch<__half>(a, s);
