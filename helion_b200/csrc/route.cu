@@ -8,15 +8,17 @@
 //   weights: the picks' scores (without the bias), divided by their sum if asked for, times scale
 //
 // Which experts come out is decided as in exact arithmetic: the fast form orders approximate choices that are off by
-// less than half of `margin` (below), and a row in which two neighbouring picks, or the last group that stays and the
-// first that goes, are closer than that is decided again in 64 bits (choose_exactly).
+// less than half of a margin (below), and a row in which two neighbouring picks, or the last group that stays and the
+// first that goes, are closer than that is decided again in 64 bits (choose_exactly), as are rows with a NaN and rows
+// that have fewer live experts than picks.
 //
 // Bound by instructions: at 65536 tokens x 256 experts the bytes take 11 us, and what a warp does per token decides.
 //  * a lane holds VPL neighbouring experts, loaded with one or two vector loads; the bias stays in registers;
-//  * choices become order-preserving 32-bit keys whose last log2(VPL) bits are replaced by the expert's place in the
-//    lane, so the key that wins a lane also says which expert it is (what the bits are worth is in the margin);
-//  * a lane keeps its two best keys; a round takes one redux over the warp, one ballot (the lowest lane wins a tie, as
-//    the lowest index must) and one shuffle, and only a lane that has given up both keys looks through its experts again;
+//  * the k best choices are no smaller than the smallest of the lanes' best ones (where more than k lanes have any):
+//    that range, [lo, hi], is spread over 22 or 23 bits, which loses no more than fp32 does, and the expert's index,
+//    counted down, takes the rest of a 32-bit key.  The largest key of the warp, one redux, then is the next pick with
+//    its index, ties going to the lowest;
+//  * a lane keeps its two best keys, and only a lane that has given up both looks through its experts again;
 //  * the picks' logits are read again at the end, by lane r for pick r, instead of travelling through the rounds.
 #include "common.cuh"
 
@@ -212,180 +214,217 @@ __device__ __noinline__ Picks choose_exactly(const Args& a, const T* row, int la
 // ------------------------------------------------------------------ fast form
 constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float redux_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float redux_min(float v) {
+  float r;
+  asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// How groups lie in the lanes: none, whole lanes (a power of two of them) per group, or anyhow.
+enum Groups { kNoGroups = 0, kLaneGroups = 1, kAnyGroups = 2 };
+
 // (the exact form, a call that few rows make, would otherwise set the registers and with them the occupancy)
-template <typename T, int VPL, bool GROUPS>
+template <typename T, int VPL, int GROUPS>
 __global__ void __launch_bounds__(kWarps * 32, VPL <= 8 ? 4 : (VPL == 16 ? 2 : 1))
 route_experts_kernel(const __grid_constant__ Args a) {
-  constexpr uint32_t kPlace = VPL - 1;  // the key bits that hold an expert's place in its lane, counted down
-  constexpr uint32_t kMasked = VPL;     // key of a masked expert: below every live one, above 0 (not to be picked)
-  __shared__ uint32_t shared_keys[GROUPS ? kWarps : 1][GROUPS ? 32 * VPL : 1];
-  uint32_t* group_keys = shared_keys[GROUPS ? threadIdx.x >> 5 : 0];
+  constexpr int kIndexBits = 5 + log2_of(VPL), kValueBits = kIndexBits <= 9 ? 23 : 32 - kIndexBits;
+  constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
+  __shared__ float shared_choices[GROUPS == kAnyGroups ? kWarps : 1][GROUPS == kAnyGroups ? 32 * VPL : 1];
+  float* my_choices = shared_choices[GROUPS == kAnyGroups ? threadIdx.x >> 5 : 0];
   const int lane = threadIdx.x & 31;
   const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr;
-  const bool by_scores = GROUPS && a.group_top > 1;  // group scores are sums of scores
-  // Half of a margin is what one choice may be off by.  Sigmoid: 7 units of 2^-24 (its argument's rounding, one
-  // exponential, one addition, one reciprocal, of values up to 1); softmax: up to 30 (the rounding of logit - top
-  // scaled by the score, the sum's own error); the bias's addition half a unit in the last place; and the place bits
-  // cut VPL units off the key.  Without a bias the logits themselves are compared.
-  const float base = !biased ? 1e-36f : (sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18));
-  auto margin = [&](float v) { return base + fabsf(v) * ((VPL + 2) * (1.f / (1 << 23))); };
+  const bool by_scores = GROUPS != kNoGroups && a.group_top > 1;  // group scores are sums of scores
+  // What two choices may be off by, together.  Sigmoid: 14 units of 2^-24 (its argument's rounding, one exponential,
+  // one addition, one reciprocal, of values up to 1, twice); softmax: up to 60 (the rounding of logit - top scaled by
+  // the score, the sum's own error, twice); additions half a unit in the last place each.  Without a bias the logits
+  // themselves are compared.
+  const float base = !biased ? 0.f : (sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18));
 
   float b[VPL];
-  bool bias_spoilt = false;
 #pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    b[j] = (biased && lane * VPL + j < a.experts) ? a.bias[lane * VPL + j] : 0.f;
-    bias_spoilt |= b[j] != b[j];
-  }
+  for (int j = 0; j < VPL; ++j) b[j] = (biased && lane * VPL + j < a.experts) ? a.bias[lane * VPL + j] : 0.f;
 
   const int64_t step = int64_t(gridDim.x) * kWarps;
   for (int64_t token = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); token < a.tokens; token += step) {
     const T* row = static_cast<const T*>(a.logits) + token * a.ld;
-    float l[VPL];
-    load_row<T, VPL>(a, row, lane, l);
-    // A NaN (or, under softmax, an infinite logit) spoils the row's scores: its weights come out as NaN.
-    bool spoilt = bias_spoilt;
-    float top = -INFINITY, total = 0.f, inv_total = 0.f;
+    float c[VPL];  // logits, then choices
+    load_row<T, VPL>(a, row, lane, c);
+    float top = c[0], low = c[0], total = 0.f, inv_total = 0.f;
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) spoilt |= l[j] != l[j] || (!sigmoid && l[j] == INFINITY);
-    spoilt = __any_sync(kAll, spoilt);
+    for (int j = 1; j < VPL; ++j) top = max_nan(top, c[j]), low = fminf(low, c[j]);
+    float hi = top;  // a lane's best choice
+    top = redux_max_nan(top);
+    // A NaN (or, under softmax, an infinite logit) spoils the row's scores: its weights come out as NaN.
+    bool spoilt = top != top || (!sigmoid && top == INFINITY);
     if (!sigmoid && (biased || by_scores || !a.renormalize)) {
 #pragma unroll
-      for (int j = 0; j < VPL; ++j) top = fmaxf(top, l[j]);
-      top = warp_max_of(top);
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) total += l[j] > -INFINITY ? exp2_fast(kLog2e * (l[j] - top)) : 0.f;
+      for (int j = 0; j < VPL; ++j) total += exp2_fast(kLog2e * (c[j] - top));
       total = warp_total(total);
       inv_total = reciprocal_fast(total);
     }
-
-    uint32_t key[VPL];
+    if (biased) {
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-      const bool live = l[j] > -INFINITY;
-      float choice = l[j];
-      if (biased) choice = live ? score_fast(l[j], sigmoid, top, inv_total) + b[j] : -INFINITY;
-      key[j] = choice > -INFINITY ? key_of(choice) : kMasked;  // (a NaN is masked)
-      if (lane * VPL + j >= a.experts) key[j] = 0;
+      for (int j = 0; j < VPL; ++j) {
+        const float score = score_fast(c[j], sigmoid, top, inv_total);
+        c[j] = low == -INFINITY && c[j] == -INFINITY ? -INFINITY : score + b[j];
+      }
+      hi = c[0];
+#pragma unroll
+      for (int j = 1; j < VPL; ++j) hi = max_nan(hi, c[j]);
+      spoilt = __any_sync(kAll, spoilt || hi != hi);
     }
-    bool unsure = false;
+    bool slow = spoilt;  // decided by choose_exactly
 
-    if constexpr (GROUPS) {
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) group_keys[lane * VPL + j] = key[j];
-      __syncwarp();
-      // 2^lanes_log lanes look through a group
+    bool alive = hi > -INFINITY;  // this lane has experts to pick
+    if constexpr (GROUPS != kNoGroups) {
+      // the two best choices of the group that this lane looks through: its own experts' group, or (any layout) one
+      // that 2^lanes_log lanes share
       const int lanes = 1 << a.lanes_log, group = lane >> a.lanes_log;
-      uint32_t m1 = 0, m2 = 0;
-      if (group < a.num_groups) {
-        for (int i = lane & (lanes - 1); i < a.group_size; i += lanes) {
-          const uint32_t k = group_keys[group * a.group_size + i];
-          m2 = max(m2, min(m1, k));
-          m1 = max(m1, k);
+      const bool is_group = group < a.num_groups;
+      float m1 = -INFINITY, m2 = -INFINITY;
+      if constexpr (GROUPS == kLaneGroups) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) m2 = fmaxf(m2, fminf(m1, c[j])), m1 = fmaxf(m1, c[j]);
+      } else {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) my_choices[lane * VPL + j] = c[j];
+        __syncwarp();
+        if (is_group) {
+          for (int i = lane & (lanes - 1); i < a.group_size; i += lanes) {
+            const float v = my_choices[group * a.group_size + i];
+            m2 = fmaxf(m2, fminf(m1, v));
+            m1 = fmaxf(m1, v);
+          }
         }
       }
       for (int o = 1; o < lanes; o <<= 1) {
-        const uint32_t o1 = __shfl_xor_sync(kAll, m1, o), o2 = __shfl_xor_sync(kAll, m2, o);
-        m2 = max(max(m2, o2), min(m1, o1));
-        m1 = max(m1, o1);
+        const float o1 = __shfl_xor_sync(kAll, m1, o), o2 = __shfl_xor_sync(kAll, m2, o);
+        m2 = fmaxf(fmaxf(m2, o2), fminf(m1, o1));
+        m1 = fmaxf(m1, o1);
       }
-      float s = -INFINITY;
-      if (m1 > kMasked) {
-        const bool convert = by_scores && !biased;
-        s = convert ? score_fast(value_of(m1), sigmoid, top, inv_total) : value_of(m1);
-        if (by_scores && m2 > kMasked) s += convert ? score_fast(value_of(m2), sigmoid, top, inv_total) : value_of(m2);
-      }
+      const bool convert = by_scores && !biased;
+      float s = m1;
+      if (convert && m1 > -INFINITY) s = score_fast(m1, sigmoid, top, inv_total);
+      if (by_scores && m2 > -INFINITY) s += convert ? score_fast(m2, sigmoid, top, inv_total) : m2;
       int before = 0;
       for (int g = 0; g < a.num_groups; ++g) {
         const float other = __shfl_sync(kAll, s, g << a.lanes_log);
         before += other > s || (other == s && g < group);
       }
-      const bool is_group = group < a.num_groups, stays = is_group && before < a.top_groups;
-      const unsigned kept = __ballot_sync(kAll, stays);
+      const bool stays = is_group && before < a.top_groups;
       if (a.top_groups < a.num_groups) {
-        const float last = value_of(~__reduce_max_sync(kAll, stays ? ~key_of(s) : 0u));
-        const float first = value_of(__reduce_max_sync(kAll, is_group && !stays ? key_of(s) : 0u));
+        const float last = redux_min(stays ? s : INFINITY), first = redux_max_nan(is_group && !stays ? s : -INFINITY);
         // sums of two are off by twice as much, and scores of logits by a softmax's margin at most
-        const float slack = by_scores ? 2.f * margin(last) + (biased ? 0.f : 1.f / (1 << 17)) : (biased ? margin(last) : 0.f);
-        unsure = first > -INFINITY && last - first <= slack && slack > 0.f;
+        const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
+        const float slack = (by_scores ? 2.f : 1.f) * (error + (error > 0.f ? fabsf(last) * (1.f / (1 << 22)) : 0.f));
+        slow |= first > -INFINITY && slack > 0.f && last - first <= slack;
       }
+      if constexpr (GROUPS == kLaneGroups) {
+        alive = alive && stays;
+        if (!alive) hi = -INFINITY;
+      } else {
+        const unsigned kept = __ballot_sync(kAll, stays);
+        hi = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const uint32_t g = (uint32_t(lane * VPL + j) * a.group_inv) >> 20;
-        if (!((kept >> ((g << a.lanes_log) & 31u)) & 1u)) key[j] = 0;
+        for (int j = 0; j < VPL; ++j) {
+          const uint32_t g = (uint32_t(lane * VPL + j) * a.group_inv) >> 20;
+          if (!((kept >> ((g << a.lanes_log) & 31u)) & 1u)) c[j] = -INFINITY;
+          hi = max_nan(hi, c[j]);
+        }
+        alive = hi > -INFINITY;
       }
     }
 
-    // a lane's two best keys, the experts' places in their last bits
-    uint32_t m1 = 0, m2 = 0;
+    // [lo, hi]: what the picks lie in
+    float lo = redux_min(alive ? hi : INFINITY);
+    hi = redux_max_nan(hi);
+    if (__popc(__ballot_sync(kAll, alive)) <= a.top_k) {  // too few lanes: the smallest live choice bounds the picks
+      lo = INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) lo = c[j] > -INFINITY ? fminf(lo, c[j]) : lo;
+      lo = redux_min(alive ? lo : INFINITY);
+    }
+    const float range = hi - lo;
+    slow |= !(range < 1e30f);
+    const float scale = float((1 << kValueBits) - 600) * reciprocal_fast(fmaxf(range, 1e-30f));
+    // value 0: below lo, masked or dropped; 1 and up: in the range.  Added to 2^23 it is the sum's last 23 bits, and
+    // what 2^23 itself would leave in the key goes with the index's constant.
+    uint32_t key[VPL], m1 = 0, m2 = 0;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-      if (key[j] != 0) key[j] = (key[j] & ~kPlace) | (kPlace - j);
+      const float q = fmaxf(fmaf(c[j] - lo, scale, 8388609.f), 8388608.f);
+      key[j] = (__float_as_uint(q) << kIndexBits) + (kIndexMask - uint32_t(lane * VPL + j) - (0x4b000000u << kIndexBits));
       m2 = max(m2, min(m1, key[j]));
       m1 = max(m1, key[j]);
     }
-    bool have2 = true;
-    uint32_t pick_key = 0, left_key = 0;
-    int pick_lane = 0, left_lane = 0;
+    if (!alive) m1 = 0;
+    uint32_t pick = 0, left = 0;
     for (int r = 0; r <= a.top_k; ++r) {  // one more, to compare the last pick with what it left behind
-      const uint32_t mine = m1 & ~kPlace, best = __reduce_max_sync(kAll, mine);
-      const int at = __ffs(__ballot_sync(kAll, mine == best)) - 1;
-      const uint32_t won = __shfl_sync(kAll, m1, at);
-      if (lane == r) pick_key = won, pick_lane = at;
-      left_key = won, left_lane = at;
-      if (lane == at) {
-        if (have2) {
+      left = __reduce_max_sync(kAll, m1);
+      if (lane == r) pick = left;
+      if (m1 == left) {
+        if (m2 != 0) {
           m1 = m2;
-          have2 = false;
+          m2 = 0;
         } else {
           m1 = 0;
 #pragma unroll
-          for (int j = 0; j < VPL; ++j) m1 = key[j] < won ? max(m1, key[j]) : m1;
+          for (int j = 0; j < VPL; ++j) m1 = key[j] < left ? max(m1, key[j]) : m1;
         }
       }
     }
-    auto expert_of = [&](uint32_t k, int at) { return at * VPL + int(kPlace - (k & kPlace)); };
-    Picks p{expert_of(pick_key, pick_lane), -INFINITY};
-    if (lane < a.top_k) p.logit = float(row[p.expert]);
-    {
-      uint32_t next_key = __shfl_down_sync(kAll, pick_key, 1);
-      if (lane == a.top_k - 1) next_key = left_key;
-      const float hi = value_of(pick_key & ~kPlace), lo = value_of(next_key & ~kPlace);
-      bool close = lane < a.top_k && (next_key & ~kPlace) > kMasked && hi - lo <= margin(hi);
+
+    const bool has_pick = lane < a.top_k;
+    slow = __any_sync(kAll, slow || (has_pick && (pick >> kIndexBits) == 0));
+    Picks p{int(kIndexMask - (pick & kIndexMask)), -INFINITY};
+    if (!slow) {
+      if (has_pick) p.logit = float(row[p.expert]);
+      uint32_t next = __shfl_down_sync(kAll, pick, 1);
+      if (lane == a.top_k - 1) next = left;
+      // in units of the keys' values: the choices' error, and two for the values' own rounding
+      const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 2.f);
+      const uint32_t gap = (pick >> kIndexBits) - (next >> kIndexBits);
+      bool close = has_pick && (next >> kIndexBits) != 0 && float(gap) <= margin;
       if (__any_sync(kAll, close)) {  // equal inputs are a tie whatever the precision
-        const int left = min(expert_of(left_key, left_lane), a.experts - 1);
-        float next_logit = __shfl_down_sync(kAll, p.logit, 1), next_bias = 0.f, bias = 0.f;
-        if (lane == a.top_k - 1) next_logit = float(row[left]);
-        if (biased) {
-          bias = a.bias[min(p.expert, a.experts - 1)];
-          next_bias = __shfl_down_sync(kAll, bias, 1);
-          if (lane == a.top_k - 1) next_bias = a.bias[left];
+        const int next_expert = int(kIndexMask - (next & kIndexMask));
+        if (close) {
+          const float bias = biased ? a.bias[p.expert] : 0.f, next_bias = biased ? a.bias[next_expert] : 0.f;
+          close = !(p.logit == float(row[next_expert]) && bias == next_bias);
         }
-        close = close && !(p.logit == next_logit && bias == next_bias);
+        slow = __any_sync(kAll, close);
       }
-      unsure = __any_sync(kAll, unsure || close);
     }
-    if (unsure && !spoilt) p = choose_exactly<T, VPL>(a, row, lane);
+    if (slow) p = choose_exactly<T, VPL>(a, row, lane);
 
     // Weights.  Renormalised ones are ratios of scores: they are formed relative to the largest pick, so that picks
     // far below the row's largest logit (a bias or a group can choose them) keep their ratios.
-    const bool live = lane < a.top_k && p.logit > -INFINITY;
+    const bool live = has_pick && p.logit > -INFINITY;
     float w = 0.f;
     if (a.renormalize) {
-      const float best = warp_max_of(live ? p.logit : -INFINITY);
+      const float best = redux_max_nan(live ? p.logit : -INFINITY);
       if (live) {
         if (!sigmoid) w = expf(p.logit - best);
-        else if (p.logit >= 0.f) w = 1.f / (1.f + expf(-p.logit));
-        else w = expf(p.logit - fminf(best, 0.f)) / (1.f + expf(p.logit));
+        else if (p.logit >= 0.f) w = __fdividef(1.f, 1.f + expf(-p.logit));
+        else w = __fdividef(expf(p.logit - fminf(best, 0.f)), 1.f + expf(p.logit));
       }
       const float sum = warp_total(w);
-      if (live) w = w / sum;
+      if (live) w = __fdividef(w, sum);
     } else if (live) {
-      w = sigmoid ? sigmoid_of(p.logit) : expf(p.logit - top) / total;
+      w = sigmoid ? sigmoid_of(p.logit) : __fdividef(expf(p.logit - top), total);
     }
     w = spoilt ? NAN : w * a.scale;
-    if (lane < a.top_k) {
+    if (has_pick) {
       a.weights[token * a.top_k + lane] = w;
       a.chosen[token * a.top_k + lane] = p.expert;
     }
@@ -398,8 +437,16 @@ int launch_vpl(Args& a, cudaStream_t s) {
   a.vec = a.experts % VPL == 0 && reinterpret_cast<uintptr_t>(a.logits) % kWord == 0 && (a.ld * int64_t(sizeof(T))) % kWord == 0;
   const int64_t blocks = (a.tokens + kWarps - 1) / kWarps;
   const int grid = int(blocks < 148 * 16 ? blocks : 148 * 16);
-  if (a.num_groups > 1) route_experts_kernel<T, VPL, true><<<grid, kWarps * 32, 0, s>>>(a);
-  else route_experts_kernel<T, VPL, false><<<grid, kWarps * 32, 0, s>>>(a);
+  const int lanes = a.group_size / VPL;
+  if (a.num_groups == 1) {
+    route_experts_kernel<T, VPL, kNoGroups><<<grid, kWarps * 32, 0, s>>>(a);
+  } else if (a.group_size % VPL == 0 && (lanes & (lanes - 1)) == 0) {
+    a.lanes_log = 0;
+    while ((1 << a.lanes_log) < lanes) ++a.lanes_log;
+    route_experts_kernel<T, VPL, kLaneGroups><<<grid, kWarps * 32, 0, s>>>(a);
+  } else {
+    route_experts_kernel<T, VPL, kAnyGroups><<<grid, kWarps * 32, 0, s>>>(a);
+  }
   return launch_status();
 }
 
