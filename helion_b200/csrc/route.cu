@@ -233,9 +233,12 @@ __device__ __forceinline__ float redux_min(float v) {
 // How groups lie in the lanes: none, whole lanes (a power of two of them) per group, or anyhow.
 enum Groups { kNoGroups = 0, kLaneGroups = 1, kAnyGroups = 2 };
 
-// (the exact form, a call that few rows make, would otherwise set the registers and with them the occupancy)
+// CTAs per SM (the exact form, a call that few rows make, would otherwise set the registers and with them the occupancy);
+// the grid is that many and every warp takes its tokens in turn, so all of them end within a token of each other.
+template <int VPL> constexpr int kResident = VPL <= 8 ? 4 : (VPL == 16 ? 2 : 1);
+
 template <typename T, int VPL, int GROUPS>
-__global__ void __launch_bounds__(kWarps * 32, VPL <= 8 ? 4 : (VPL == 16 ? 2 : 1))
+__global__ void __launch_bounds__(kWarps * 32, kResident<VPL>)
 route_experts_kernel(const __grid_constant__ Args a) {
   constexpr int kIndexBits = 5 + log2_of(VPL), kValueBits = kIndexBits <= 9 ? 23 : 32 - kIndexBits;
   constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
@@ -259,30 +262,37 @@ route_experts_kernel(const __grid_constant__ Args a) {
     const T* row = static_cast<const T*>(a.logits) + token * a.ld;
     float c[VPL];  // logits, then choices
     load_row<T, VPL>(a, row, lane, c);
-    float top = c[0], low = c[0], total = 0.f, inv_total = 0.f;
+    float top = 0.f, total = 0.f, inv_total = 0.f;
+    float hi = c[0];  // a lane's best choice
 #pragma unroll
-    for (int j = 1; j < VPL; ++j) top = max_nan(top, c[j]), low = fminf(low, c[j]);
-    float hi = top;  // a lane's best choice
-    top = redux_max_nan(top);
+    for (int j = 1; j < VPL; ++j) hi = max_nan(hi, c[j]);
     // A NaN (or, under softmax, an infinite logit) spoils the row's scores: its weights come out as NaN.
-    bool spoilt = top != top || (!sigmoid && top == INFINITY);
-    if (!sigmoid && (biased || by_scores || !a.renormalize)) {
+    bool spoilt = false;
+    if (!sigmoid) {
+      top = redux_max_nan(hi);
+      spoilt = top == INFINITY;
+      if (biased || by_scores || !a.renormalize) {
 #pragma unroll
-      for (int j = 0; j < VPL; ++j) total += exp2_fast(kLog2e * (c[j] - top));
-      total = warp_total(total);
-      inv_total = reciprocal_fast(total);
+        for (int j = 0; j < VPL; ++j) total += exp2_fast(kLog2e * (c[j] - top));
+        total = warp_total(total);
+        inv_total = reciprocal_fast(total);
+      }
     }
     if (biased) {
+      float low = c[0];
 #pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const float score = score_fast(c[j], sigmoid, top, inv_total);
-        c[j] = low == -INFINITY && c[j] == -INFINITY ? -INFINITY : score + b[j];
+      for (int j = 1; j < VPL; ++j) low = fminf(low, c[j]);
+      float choice[VPL];
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) choice[j] = score_fast(c[j], sigmoid, top, inv_total) + b[j];
+      if (low == -INFINITY) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) choice[j] = c[j] == -INFINITY ? -INFINITY : choice[j];
       }
-      hi = c[0];
 #pragma unroll
-      for (int j = 1; j < VPL; ++j) hi = max_nan(hi, c[j]);
-      spoilt = __any_sync(kAll, spoilt || hi != hi);
+      for (int j = 0; j < VPL; ++j) c[j] = choice[j], hi = j == 0 ? c[0] : max_nan(hi, c[j]);
     }
+    spoilt = __any_sync(kAll, spoilt || hi != hi);
     bool slow = spoilt;  // decided by choose_exactly
 
     bool alive = hi > -INFINITY;  // this lane has experts to pick
@@ -317,18 +327,19 @@ route_experts_kernel(const __grid_constant__ Args a) {
       float s = m1;
       if (convert && m1 > -INFINITY) s = score_fast(m1, sigmoid, top, inv_total);
       if (by_scores && m2 > -INFINITY) s += convert ? score_fast(m2, sigmoid, top, inv_total) : m2;
+      // a group's rank: its score's key with the group, counted down, in the last five bits
+      const uint32_t s_key = is_group ? (key_of(s) & ~31u) | uint32_t(31 - group) : 0u;
       int before = 0;
-      for (int g = 0; g < a.num_groups; ++g) {
-        const float other = __shfl_sync(kAll, s, g << a.lanes_log);
-        before += other > s || (other == s && g < group);
-      }
+#pragma unroll 4
+      for (int g = 0; g < a.num_groups; ++g) before += __shfl_sync(kAll, s_key, g << a.lanes_log) > s_key;
       const bool stays = is_group && before < a.top_groups;
       if (a.top_groups < a.num_groups) {
         const float last = redux_min(stays ? s : INFINITY), first = redux_max_nan(is_group && !stays ? s : -INFINITY);
-        // sums of two are off by twice as much, and scores of logits by a softmax's margin at most
+        // sums of two are off by twice as much, scores of logits by a softmax's margin at most, and the five bits are
+        // 2^-18 of a score; 16-bit logits lose nothing to them
         const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
-        const float slack = (by_scores ? 2.f : 1.f) * (error + (error > 0.f ? fabsf(last) * (1.f / (1 << 22)) : 0.f));
-        slow |= first > -INFINITY && slack > 0.f && last - first <= slack;
+        const bool exact = error == 0.f && sizeof(T) == 2;
+        slow |= !exact && first > -INFINITY && last - first <= 2.f * error + fabsf(last) * (1.f / (1 << 17)) + 1e-36f;
       }
       if constexpr (GROUPS == kLaneGroups) {
         alive = alive && stays;
@@ -373,15 +384,12 @@ route_experts_kernel(const __grid_constant__ Args a) {
     for (int r = 0; r <= a.top_k; ++r) {  // one more, to compare the last pick with what it left behind
       left = __reduce_max_sync(kAll, m1);
       if (lane == r) pick = left;
-      if (m1 == left) {
-        if (m2 != 0) {
-          m1 = m2;
-          m2 = 0;
-        } else {
-          m1 = 0;
+      const bool mine = m1 == left;
+      m1 = mine ? m2 : m1;
+      m2 = mine ? 0 : m2;
+      if (mine && m1 == 0) {  // both given up
 #pragma unroll
-          for (int j = 0; j < VPL; ++j) m1 = key[j] < left ? max(m1, key[j]) : m1;
-        }
+        for (int j = 0; j < VPL; ++j) m1 = key[j] < left ? max(m1, key[j]) : m1;
       }
     }
 
@@ -413,10 +421,14 @@ route_experts_kernel(const __grid_constant__ Args a) {
     float w = 0.f;
     if (a.renormalize) {
       const float best = redux_max_nan(live ? p.logit : -INFINITY);
-      if (live) {
-        if (!sigmoid) w = expf(p.logit - best);
-        else if (p.logit >= 0.f) w = __fdividef(1.f, 1.f + expf(-p.logit));
-        else w = __fdividef(expf(p.logit - fminf(best, 0.f)), 1.f + expf(p.logit));
+      if (!sigmoid) {
+        w = live ? expf(p.logit - best) : 0.f;
+      } else {
+        // relative to the best pick's exp(best) where that is negative
+        const float t = expf(-fabsf(p.logit));
+        float numerator = p.logit < 0.f ? t : 1.f;
+        if (best < 0.f) numerator = expf(p.logit - best);
+        w = live ? __fdividef(numerator, 1.f + t) : 0.f;
       }
       const float sum = warp_total(w);
       if (live) w = __fdividef(w, sum);
@@ -436,7 +448,8 @@ int launch_vpl(Args& a, cudaStream_t s) {
   constexpr int kBytes = VPL * int(sizeof(T)), kWord = kBytes < 16 ? kBytes : 16;
   a.vec = a.experts % VPL == 0 && reinterpret_cast<uintptr_t>(a.logits) % kWord == 0 && (a.ld * int64_t(sizeof(T))) % kWord == 0;
   const int64_t blocks = (a.tokens + kWarps - 1) / kWarps;
-  const int grid = int(blocks < 148 * 16 ? blocks : 148 * 16);
+  const int64_t places = int64_t(kResident<VPL>) * 148;
+  const int grid = int(blocks < places ? blocks : places);
   const int lanes = a.group_size / VPL;
   if (a.num_groups == 1) {
     route_experts_kernel<T, VPL, kNoGroups><<<grid, kWarps * 32, 0, s>>>(a);
