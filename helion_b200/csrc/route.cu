@@ -8,9 +8,11 @@
 //   weights: the picks' scores (without the bias), divided by their sum if asked for, times scale
 //
 // Which experts come out is decided as in exact arithmetic: the fast form orders approximate choices that are off by
-// less than half of a margin (below), and a row in which two neighbouring picks, or the last group that stays and the
-// first that goes, are closer than that is decided again in 64 bits (choose_exactly), as are rows with a NaN and rows
-// that have fewer live experts than picks.
+// less than half of a margin (below), and where two neighbouring picks, or the last group that stays and the first that
+// goes, are closer than that, those picks (refine_picks) or groups (refine_groups) are compared again in 64 bits: about
+// two rows in a thousand, and what a refinement takes is part of every larger call's time.  Rows with a NaN, rows that
+// have fewer live experts than picks and the rare row in which the candidates themselves are unsure are decided in 64
+// bits from the start (choose_exactly).
 //
 // Bound by instructions: at 65536 tokens x 256 experts the bytes take 11 us, and what a warp does per token decides.
 //  * a lane holds VPL neighbouring experts, loaded with one or two vector loads; the bias stays in registers;
@@ -37,6 +39,7 @@ struct Args {
   int experts, top_k, sigmoid, num_groups, top_groups, group_top, group_size, renormalize;
   int vec;            // a lane's experts can be read with vector loads
   int lanes_log;      // log2 of the lanes that look through a group
+  uint32_t group_low; // 2^b - 1 >= num_groups - 1: the last b bits of a group score's key hold the group
   uint32_t group_inv; // ceil(2^20 / group_size): e / group_size = e * group_inv >> 20 for e < 1024
   float scale;
 };
@@ -109,6 +112,85 @@ struct Picks {
   int expert;   // lane r holds pick r
   float logit;
 };
+
+// ------------------------------------------------------------------ 64-bit comparisons of what fp32 leaves unsure
+// The softmax's sum, where an exact choice needs it (1 otherwise: it would scale both sides of a comparison).
+template <typename T>
+__device__ __forceinline__ double exact_total(const Args& a, const T* row, float top, int lane) {
+  if (a.sigmoid || a.bias == nullptr) return 1.0;
+  double total = 0.0;
+  for (int e = lane; e < a.experts; e += 32) {
+    const float l = float(row[e]);
+    if (l > -INFINITY) total += exp(double(l) - double(top));
+  }
+  return warp_total(total);
+}
+
+// Score (of_score) or logit, plus the bias.
+__device__ __forceinline__ double exact_choice(const Args& a, float logit, int e, float top, double total, bool of_score) {
+  double c = double(logit);
+  if (of_score) {
+    const double t = a.sigmoid ? exp(-fabs(c)) : exp(c - double(top));
+    c = a.sigmoid ? (c < 0.0 ? t : 1.0) / (1.0 + t) : t / total;
+  }
+  return a.bias != nullptr ? c + double(a.bias[e]) : c;
+}
+
+// Whether the group of this lane stays.  `sure`: its approximate score lies clear above the undecided ones; `near`: it
+// is one of these, and is compared by its exact score.
+template <typename T>
+__device__ __noinline__ bool refine_groups(const Args& a, const T* row, float top, int group, bool sure, bool near) {
+  const int lane = threadIdx.x & 31, lanes = 1 << a.lanes_log;
+  const bool of_score = a.bias != nullptr || a.group_top > 1;
+  const double total = exact_total(a, row, top, lane);
+  const unsigned near_lanes = __ballot_sync(kAll, near);
+  const int sure_groups = __popc(__ballot_sync(kAll, sure && (lane & (lanes - 1)) == 0));
+  double mine = -INFINITY;
+  for (int g = 0; g < a.num_groups; ++g) {
+    if (!((near_lanes >> (g << a.lanes_log)) & 1u)) continue;
+    double b1 = -INFINITY, b2 = -INFINITY;
+    for (int i = lane; i < a.group_size; i += 32) {
+      const int e = g * a.group_size + i;
+      const float l = float(row[e]);
+      if (!(l > -INFINITY)) continue;
+      const double c = exact_choice(a, l, e, top, total, of_score);
+      if (c > b1) b2 = b1, b1 = c; else if (c > b2) b2 = c;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const double o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
+      const double low = o1 < b1 ? o1 : b1, high = o1 < b1 ? b1 : o1, second = o2 < b2 ? b2 : o2;
+      b1 = high;
+      b2 = low > second ? low : second;
+    }
+    if (group == g) mine = a.group_top > 1 && b2 > -INFINITY ? b1 + b2 : b1;
+  }
+  int before = 0;
+  for (int g = 0; g < a.num_groups; ++g) {
+    const double other = __shfl_sync(kAll, mine, g << a.lanes_log);
+    if ((near_lanes >> (g << a.lanes_log)) & 1u) before += other > mine || (other == mine && g < group);
+  }
+  return sure || (near && before < a.top_groups - sure_groups);
+}
+
+// The picks of lanes 0 .. count - 1 in the order of their exact choices.
+template <typename T>
+__device__ __noinline__ Picks refine_picks(const Args& a, const T* row, float top, Picks p, int count) {
+  const int lane = threadIdx.x & 31;
+  const bool has = lane < count;
+  const double total = exact_total(a, row, top, lane);
+  const double mine = has ? exact_choice(a, p.logit, p.expert, top, total, a.bias != nullptr) : 0.0;
+  int rank = 0;
+  for (int r = 0; r < count; ++r) {
+    const double other = __shfl_sync(kAll, mine, r);
+    const int expert = __shfl_sync(kAll, p.expert, r);
+    rank += other > mine || (other == mine && expert < p.expert);
+  }
+  int from = lane;
+  for (int r = 0; r < count; ++r)
+    if (__shfl_sync(kAll, rank, r) == lane) from = r;
+  return Picks{__shfl_sync(kAll, p.expert, from), __shfl_sync(kAll, p.logit, from)};
+}
 
 // ------------------------------------------------------------------ exact form, for the few rows that need it
 __device__ __forceinline__ double warp_best(double v) {
@@ -327,19 +409,21 @@ route_experts_kernel(const __grid_constant__ Args a) {
       float s = m1;
       if (convert && m1 > -INFINITY) s = score_fast(m1, sigmoid, top, inv_total);
       if (by_scores && m2 > -INFINITY) s += convert ? score_fast(m2, sigmoid, top, inv_total) : m2;
-      // a group's rank: its score's key with the group, counted down, in the last five bits
-      const uint32_t s_key = is_group ? (key_of(s) & ~31u) | uint32_t(31 - group) : 0u;
+      // a group's rank: its score's key with the group, counted down, in the last bits
+      const uint32_t s_key = is_group ? (key_of(s) & ~a.group_low) | (a.group_low - uint32_t(group)) : 0u;
       int before = 0;
 #pragma unroll 4
       for (int g = 0; g < a.num_groups; ++g) before += __shfl_sync(kAll, s_key, g << a.lanes_log) > s_key;
-      const bool stays = is_group && before < a.top_groups;
+      bool stays = is_group && before < a.top_groups;
       if (a.top_groups < a.num_groups) {
         const float last = redux_min(stays ? s : INFINITY), first = redux_max_nan(is_group && !stays ? s : -INFINITY);
-        // sums of two are off by twice as much, scores of logits by a softmax's margin at most, and the five bits are
-        // 2^-18 of a score; 16-bit logits lose nothing to them
+        // sums of two are off by twice as much, scores of logits by a softmax's margin at most, and the key's last bits
+        // are (group_low + 1) 2^-23 of a score; 16-bit logits lose nothing to them
         const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
         const bool exact = error == 0.f && sizeof(T) == 2;
-        slow |= !exact && first > -INFINITY && last - first <= 2.f * error + fabsf(last) * (1.f / (1 << 17)) + 1e-36f;
+        const float slack = 2.f * error + fabsf(last) * (float(a.group_low + 3) * (1.f / (1 << 22))) + 1e-36f;
+        if (!exact && first > -INFINITY && last - first <= slack && !spoilt)
+          stays = refine_groups<T>(a, row, top, group, is_group && s > last + slack, is_group && s >= first - slack && s <= last + slack);
       }
       if constexpr (GROUPS == kLaneGroups) {
         alive = alive && stays;
@@ -402,15 +486,24 @@ route_experts_kernel(const __grid_constant__ Args a) {
       if (lane == a.top_k - 1) next = left;
       // in units of the keys' values: the choices' error, and two for the values' own rounding
       const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 2.f);
-      const uint32_t gap = (pick >> kIndexBits) - (next >> kIndexBits);
-      bool close = has_pick && (next >> kIndexBits) != 0 && float(gap) <= margin;
-      if (__any_sync(kAll, close)) {  // equal inputs are a tie whatever the precision
-        const int next_expert = int(kIndexMask - (next & kIndexMask));
-        if (close) {
-          const float bias = biased ? a.bias[p.expert] : 0.f, next_bias = biased ? a.bias[next_expert] : 0.f;
-          close = !(p.logit == float(row[next_expert]) && bias == next_bias);
+      bool close = has_pick && (next >> kIndexBits) != 0 && float((pick >> kIndexBits) - (next >> kIndexBits)) <= margin;
+      if (__any_sync(kAll, close)) {
+        if (close) {  // equal inputs are a tie whatever the precision
+          const int e = int(kIndexMask - (next & kIndexMask));
+          const float bias = biased ? a.bias[p.expert] : 0.f, next_bias = biased ? a.bias[e] : 0.f;
+          close = !(p.logit == float(row[e]) && bias == next_bias);
         }
-        slow = __any_sync(kAll, close);
+        const unsigned pairs = __ballot_sync(kAll, close);
+        if (pairs != 0) {
+          int count = a.top_k;
+          if ((pairs >> (a.top_k - 1)) & 1u) {  // the last pick and the one left behind: that one takes part too
+            const uint32_t beyond = __reduce_max_sync(kAll, m1);
+            count = a.top_k + 1;
+            slow = count > 32 || ((beyond >> kIndexBits) != 0 && float((left >> kIndexBits) - (beyond >> kIndexBits)) <= margin);
+            if (lane == a.top_k) p.expert = int(kIndexMask - (left & kIndexMask)), p.logit = float(row[p.expert]);
+          }
+          if (!slow) p = refine_picks<T>(a, row, top, p, count);
+        }
       }
     }
     if (slow) p = choose_exactly<T, VPL>(a, row, lane);
@@ -506,6 +599,7 @@ extern "C" int hb200_moe_route_experts(const hb200_route_args* args, void* strea
   a.scale = scale;
   a.lanes_log = 0;
   while ((num_groups << (a.lanes_log + 1)) <= 32) ++a.lanes_log;
+  while (int(a.group_low) < a.num_groups - 1) a.group_low = 2 * a.group_low + 1;
   a.group_inv = uint32_t(((1 << 20) + a.group_size - 1) / a.group_size);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (logits_dtype == 0) return route::launch<__nv_bfloat16>(a, s);
