@@ -8,10 +8,14 @@
 // up rows when gated) by up to 256 rows of x, and the accumulator holds y transposed (lane = weight row, column =
 // row of x).  A decode step is bound by the weight's bytes, and one SM streams about 1/148 of the HBM bandwidth, so
 // the K range of a tile is split over a thread-block cluster of up to 8 CTAs until there are two CTAs for every SM
-// (one, where a tile is wider than 64 rows of x).  The partial sums meet in distributed shared memory: column c of the tile belongs to rank c % split, every
-// rank stores its fp32 partial of a column into the owner's shared memory, and after one cluster barrier the owner
-// adds them in rank order (ascending K: the result does not depend on timing) and runs the epilogue.  No workspace,
-// no counters, no atomics: calls on any streams and replays of any graphs are independent of each other.
+// (one, where a tile is wider than 64 rows of x).  The partial sums meet in distributed shared memory: column c of the
+// tile belongs to rank c % split, every rank stores its fp32 partial of a column into the owner's shared memory, and
+// after one cluster barrier the owner adds them in rank order (ascending K: the result does not depend on timing) and
+// runs the epilogue.  No workspace, no counters, no atomics: calls on any streams and replays of any graphs are
+// independent of each other.  Measured: one row, 8192 x 28672, 72.8 us = 6.45 TB/s; 16 rows, gated 57344 x 8192,
+// 149.5 us = 6.29 TB/s (the copy bandwidth of this GPU is 6.54).
+//
+// linear_pair_kernel takes over where x has more rows than that form can hide behind the weight (see plan_pair).
 //
 // CTAs of 192 threads: warp 0 TMA producer (128-byte swizzle, no multicast), warp 1 MMA issuer, warps 2-5 move the
 // accumulator out of tensor memory; all six run the epilogue.  Every wait is bounded.
@@ -235,8 +239,8 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   const int tile = int(blockIdx.x) / split;
   const int m0 = (tile % g.m_chunks) * g.cols, n0 = (tile / g.m_chunks) * kOutRows;
   const int kb0 = range_start(rank, g.num_kb, split), kb1 = range_start(rank + 1, g.num_kb, split);
-  const int per = (g.cols + split - 1) / split; // columns this rank owns, at most
-  const int live_cols = min(g.cols, g.m - m0); // columns past the last row of x are never stored
+  const int per = (g.cols + split - 1) / split;  // columns this rank owns, at most
+  const int live_cols = min(g.cols, g.m - m0);   // columns past the last row of x are never stored
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.stages; ++s) {
@@ -390,7 +394,9 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // one accumulator lane 128 columns apart).  CTA r of the pair loads its 128 rows of x and its 128 weight rows, the
 // leader issues 256 x 256 x 16 MMAs (cta_group::2) that read both: per 64 elements of K every SM pulls 32 KB from L2
 // for 512 clocks of tensor work.  Two accumulators in tensor memory, so a tile's epilogue runs beside the next
-// tile's MMAs; the grid is persistent.
+// tile's MMAs; the grid is persistent.  At 8192^3 the tensor pipe is 98 % active and the GPU's power limit sets the
+// time: 1.30 PFLOP/s in sequence, 1.58 in a single launch.  Tiles of 512 x 256 (a quarter fewer bytes out of L2 per
+// product) measured 1 to 3 % faster there and up to 15 % slower at K = 1024, where their epilogue shows: not taken.
 //
 // Epilogue: sixteen warps per CTA, each 32 rows by 64 accumulator columns (gated: 32 gate and 32 up columns), a lane
 // per row.  Outputs leave through boxes of 32 rows x 64 bytes in shared memory, two per warp in turn, by TMA where the
@@ -398,10 +404,10 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // the same boxes.  Measured at 4096 x 16384 x 1024, where the epilogue shows, SiLU and residual: 151 us; a lane reading
 // and writing its own row in 32-byte sectors 167; one box per warp and a sixth stage in its place 165 (the two are level
 // from K = 4096 on).
-constexpr int kPairThreads = 576;  // producer, MMA issuer, sixteen epilogue warps
+constexpr int kPairThreads = 576;              // producer, MMA issuer, sixteen epilogue warps
 constexpr int kPairTile = 256;                 // rows of x per tile
 constexpr int kHalfBytes = 128 * 128;          // 128 rows of x (or of the weight) x 64 elements of K
-constexpr int kPairRingBytes = 10 * kHalfBytes; // 160 KB: five or six stages
+constexpr int kPairRingBytes = 10 * kHalfBytes;  // 160 KB: five or six stages
 constexpr int kPairMaxStages = 6;
 constexpr int kBoxBytes = 2048;                // two boxes per epilogue warp
 constexpr int kEpilogueWarps = 16;
@@ -517,7 +523,8 @@ __device__ __forceinline__ void cluster_wait_all() { asm volatile("barrier.clust
 // share of K, and the partial sums meet in distributed shared memory: of the four groups of 64 accumulator columns that
 // a CTA's epilogue warps hold, pair q finishes groups [4 q / split, 4 (q + 1) / split) and receives the others' partials
 // of these, of its own 128 rows, in the place of the ring that all MMAs have read.  They are added in the order of the
-// pairs (own first), so the result does not depend on timing.
+// pairs (own first), so the result does not depend on timing.  200 x 8192 x 8192: 33.7 us with two pairs per tile, 51
+// with one, 42 in the streaming form.
 template <typename T, typename OutT, bool GATED, bool SPLIT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,

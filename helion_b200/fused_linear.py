@@ -27,7 +27,12 @@ _ACTIVATIONS = {
     "gelu_and_mul": (3, True),
     "gelu_tanh_and_mul": (4, True),
 }
+_cuda_getDevice = getattr(torch._C, "_cuda_getDevice", None)  # (absent in a build without CUDA, where nothing gets there)
+_cuda_getCurrentRawStream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _ARGS = struct.Struct("=12q6i")  # hb200_linear_args (a bytes object passes through ctypes at a fifth of 18 values' cost)
+
+
+_pack = _ARGS.pack
 
 
 def _check(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
@@ -83,49 +88,54 @@ def _tma_rows(t: Tensor, rows: int, k: int) -> tuple[Tensor, int, int]:
     return t, pitch, address
 
 
+_entry = None
+
+
 def _linear_cuda(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
                  out_dtype: torch.dtype) -> Tensor:
+    global _entry
     n = _check(x, weight, bias, residual, activation, out_dtype)
-    _require_cuda(x)
-    x_shape = x.shape
-    out = x.new_empty((*x_shape[:-1], n), dtype=out_dtype)
-    if out.numel() == 0:
-        return out
+    if not x.is_cuda:
+        _require_cuda(x)
     index = x.get_device()
-    if torch._C._cuda_getDevice() != index:
+    if _cuda_getDevice() != index:
         with torch.cuda.device(index):
-            _launch(out, x, weight, bias, residual, activation, n, index)
+            return _linear_cuda(x, weight, bias, residual, activation, out_dtype)
+    x_shape = x.shape
+    if len(x_shape) == 2:
+        m, k = x_shape
+        out = x.new_empty((m, n), dtype=out_dtype)
     else:
-        _launch(out, x, weight, bias, residual, activation, n, index)
-    return out
-
-
-def _launch(out: Tensor, x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str, n: int,
-            index: int) -> None:
-    rows, k = weight.shape
-    if x.dim() != 2:
+        out = x.new_empty((*x_shape[:-1], n), dtype=out_dtype)
+        k = x_shape[-1]
         x = x.reshape(-1, k)
-    m = x.shape[0]
+        m = x.shape[0]
+    if m == 0 or n == 0:
+        return out
     x, ldx, x_ptr = _tma_rows(x, m, k)
-    weight, ldw, w_ptr = _tma_rows(weight, rows, k)
+    weight, ldw, w_ptr = _tma_rows(weight, weight.shape[0], k)
     ldr = res_ptr = bias_ptr = 0
     if residual is not None:
         if residual.dim() != 2:
             residual = residual.reshape(m, n)
-        if n > 1 and residual.stride(1) != 1:
+        ldr, unit = residual.stride()
+        if unit != 1 and n > 1:
             residual = residual.contiguous()
-        ldr, res_ptr = residual.stride(0), residual.data_ptr()
+            ldr = n
+        res_ptr = residual.data_ptr()
     bias_f32 = False
     if bias is not None:
         bias = bias.contiguous()
         bias_ptr, bias_f32 = bias.data_ptr(), bias.dtype is torch.float32
     code, gated = _ACTIVATIONS[activation]
-    _lib.call(
-        "hb200_linear",
-        _ARGS.pack(x_ptr, w_ptr, bias_ptr, res_ptr, out.data_ptr(), m, n, k, ldx, ldw, ldr, n, code, gated,
-                   x.dtype is torch.bfloat16, bias_f32, out.dtype is torch.float32, 0),
-        torch._C._cuda_getCurrentRawStream(index),
+    if _entry is None:
+        _entry = _lib.entry("hb200_linear")
+    _entry(
+        _pack(x_ptr, w_ptr, bias_ptr, res_ptr, out.data_ptr(), m, n, k, ldx, ldw, ldr, n, code, gated,
+              x.dtype is torch.bfloat16, bias_f32, out_dtype is torch.float32, 0),
+        _cuda_getCurrentRawStream(index),
     )
+    return out
 
 
 @torch.library.custom_op("helion_b200::linear", mutates_args=())

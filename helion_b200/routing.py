@@ -9,6 +9,8 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .fused_linear import _cuda_getCurrentRawStream
+from .fused_linear import _cuda_getDevice
 from .fused_linear import _direct
 from .ops import _require_cuda
 
@@ -46,28 +48,40 @@ def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None,
             raise ValueError(f"all tensors must be on one device, got {router_logits.device} and {bias.device}")
 
 
+_entry = None
+
+
 def _route_cuda(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
                 group_top: int, renormalize: bool, scale: float) -> tuple[Tensor, Tensor]:
+    global _entry
     _check(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top)
-    _require_cuda(router_logits)
+    if not router_logits.is_cuda:
+        _require_cuda(router_logits)
+    index = router_logits.get_device()
+    if _cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return _route_cuda(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
     tokens, experts = router_logits.shape
     weights = router_logits.new_empty((tokens, top_k), dtype=torch.float32)
     chosen = router_logits.new_empty((tokens, top_k), dtype=torch.int64)
     if tokens == 0:
         return weights, chosen
-    if experts > 1 and router_logits.stride(1) != 1:
+    pitch, unit = router_logits.stride()
+    if unit != 1 and experts > 1:
         router_logits = router_logits.contiguous()
+        pitch = experts
+    bias_ptr = 0
     if bias is not None:
         bias = bias.contiguous()
-    args = _ARGS.pack(router_logits.data_ptr(), 0 if bias is None else bias.data_ptr(), weights.data_ptr(), chosen.data_ptr(),
-                      tokens, experts, router_logits.stride(0), top_k, num_groups, top_groups, group_top,
-                      _LOGIT_DTYPES[router_logits.dtype], _SCORINGS[scoring], renormalize, scale)
-    index = router_logits.get_device()
-    if torch._C._cuda_getDevice() != index:
-        with torch.cuda.device(index):
-            _lib.call("hb200_moe_route_experts", args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        _lib.call("hb200_moe_route_experts", args, torch._C._cuda_getCurrentRawStream(index))
+        bias_ptr = bias.data_ptr()
+    if _entry is None:
+        _entry = _lib.entry("hb200_moe_route_experts")
+    _entry(
+        _ARGS.pack(router_logits.data_ptr(), bias_ptr, weights.data_ptr(), chosen.data_ptr(), tokens, experts, pitch, top_k,
+                   num_groups, top_groups, group_top, _LOGIT_DTYPES[router_logits.dtype], _SCORINGS[scoring], renormalize,
+                   scale),
+        _cuda_getCurrentRawStream(index),
+    )
     return weights, chosen
 
 

@@ -126,18 +126,88 @@ def test_choices_closer_than_fp32_can_tell(scoring):
     assert flips > 0  # the case is one that fp32 alone gets wrong
 
 
-def test_nan_and_infinite_logits():
-    logits = torch.randn(6, 96, device=DEV)
+@pytest.mark.parametrize("experts,kw", [(64, dict(scoring="sigmoid")), (200, dict(scoring="softmax", renormalize=True)),
+                                        (64, dict(scoring="sigmoid", num_groups=8, top_groups=4, group_top=2)),
+                                        (96, dict(scoring="softmax", num_groups=4, top_groups=3))])
+def test_two_neighbouring_picks_closer_than_fp32_can_tell(experts, kw):
+    """One pair of choices, at every place among the picks and across their end, made to meet to within 2^-25."""
+    g = torch.Generator().manual_seed(experts)
+    rows, biases = [], []
+    k = 6
+    for trial in range(80):
+        logits = torch.randn(experts, generator=g)
+        bias = torch.randn(experts, generator=g) * 0.2
+        score = torch.softmax(logits.double(), 0) if kw["scoring"] == "softmax" else torch.sigmoid(logits.double())
+        order = (score + bias.double()).sort(descending=True).indices
+        i = trial % (k + 1)
+        hi, lo = order[i], order[i + 1]
+        bias[lo] = (score[hi] + bias[hi].double() - score[lo]).float()  # exact but for the bias's own rounding
+        rows.append(logits), biases.append(bias)
+    flips = 0
+    for logits, bias in zip(rows, biases):
+        _, e = compare(logits[None].to(DEV), k, bias=bias.to(DEV), **kw)
+        fp32 = (torch.softmax(logits, 0) if kw["scoring"] == "softmax" else torch.sigmoid(logits)) + bias
+        flips += fp32.sort(descending=True, stable=True).indices[:k].tolist() != e[0].tolist()
+    assert flips > 0
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,biased", [(64, 8, True), (60, 6, True), (256, 8, True), (64, 8, False), (60, 6, False)])
+def test_neighbouring_groups_closer_than_fp32_can_tell(experts, groups, biased, scoring):
+    """The last group that stays and the first that goes meet to within a rounding, in sums of two choices."""
+    g = torch.Generator().manual_seed(experts + groups)
+    size, keep = experts // groups, groups // 2
+    for trial in range(30):
+        logits = torch.randn(experts, generator=g)
+        bias = torch.randn(experts, generator=g) * 0.1 if biased else None
+        score = torch.softmax(logits.double(), 0) if scoring == "softmax" else torch.sigmoid(logits.double())
+        choice = (score + bias.double() if biased else score).view(groups, size)
+        best = choice.sort(1, descending=True).values[:, :2].sum(1)
+        order = best.sort(descending=True).indices
+        a, b = order[keep - 1], order[keep]
+        if biased:
+            top = int(choice[b].argmax()) + int(b) * size
+            bias[top] = (bias[top].double() + best[a] - best[b]).float()
+        else:  # the same two logits in both groups, in other places: a tie, and a last-place step away from one
+            pair = logits.view(groups, size)[a].sort(descending=True).values[:2]
+            logits.view(groups, size)[b] = -3.0
+            logits.view(groups, size)[b, 1], logits.view(groups, size)[b, 3] = pair[1], pair[0]
+            if trial % 3:
+                step = torch.tensor(math.inf if trial % 3 == 1 else -math.inf)
+                logits.view(groups, size)[b, 3] = torch.nextafter(pair[0], step)
+        kw = dict(scoring=scoring, num_groups=groups, top_groups=keep, group_top=2)
+        compare(logits[None].to(DEV), 5, bias=None if bias is None else bias.to(DEV), **kw)
+        compare(logits[None].to(DEV), 5, bias=None if bias is None else bias.to(DEV), **{**kw, "group_top": 1})
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_nan_and_infinite_logits(seed):
+    logits = torch.randn(6, 96, generator=torch.Generator().manual_seed(seed)).to(DEV)
     logits[1, 7] = math.nan
     logits[2] = math.nan
     logits[3, 9] = math.inf
     for scoring in ("softmax", "sigmoid"):
-        for kw in ({}, dict(num_groups=8, top_groups=3, group_top=2), dict(bias=torch.zeros(96, device=DEV), renormalize=True)):
+        for kw in ({}, dict(num_groups=8, top_groups=3, group_top=2), dict(num_groups=6, top_groups=2),
+                   dict(bias=torch.zeros(96, device=DEV), renormalize=True)):
             w, e = hb.route_experts(logits, 6, scoring=scoring, **kw)
             assert torch.isnan(w[1]).all() and torch.isnan(w[2]).all()
-            assert torch.isnan(w[3]).all() if scoring == "softmax" else (w[3] == w[3]).all() and e[3, 0] == 9
+            if scoring == "softmax":
+                assert torch.isnan(w[3]).all()
+            else:  # a score of 1, whatever the group makes of it
+                assert torch.equal(e[3:4].cpu(), route(logits[3:4], 6, scoring=scoring, **kw)[1]) and torch.isfinite(w[3]).all()
             assert torch.isfinite(w[[0, 4, 5]]).all()
             assert ((e >= 0) & (e < 96)).all() and all(len(set(r)) == 6 for r in e.tolist())
+    bias = torch.zeros(96, device=DEV)
+    bias[40] = math.nan
+    for kw in ({}, dict(num_groups=8, top_groups=1), dict(num_groups=6, top_groups=2, group_top=2)):
+        w, e = hb.route_experts(logits, 6, scoring="sigmoid", bias=bias, **kw)
+        assert torch.isnan(w).all() and all(len(set(r)) == 6 for r in e.tolist())
+    # infinite biases force an expert in or keep it out
+    bias[40], bias[41] = math.inf, -math.inf
+    clean = torch.randn(6, 96, generator=torch.Generator().manual_seed(seed + 50)).to(DEV)
+    for kw in ({}, dict(num_groups=8, top_groups=2), dict(num_groups=6, top_groups=2, group_top=2)):
+        w, e = compare(clean, 6, scoring="sigmoid", bias=bias, **kw)
+        assert (e[:, 0] == 40).all() and (e != 41).all()
 
 
 def test_strides_empty_and_repeat():
