@@ -39,6 +39,7 @@ struct Args {
   int experts, top_k, sigmoid, num_groups, top_groups, group_top, group_size, renormalize;
   int vec;            // a lane's experts can be read with vector loads
   int lanes_log;      // log2 of the lanes that look through a group
+  int many_lanes_log; // the same where eight lanes hold a token
   uint32_t group_low; // 2^b - 1 >= num_groups - 1: the last b bits of a group score's key hold the group
   uint32_t group_inv; // ceil(2^20 / group_size): e / group_size = e * group_inv >> 20 for e < 1024
   float scale;
@@ -312,8 +313,232 @@ __device__ __forceinline__ float redux_min(float v) {
   return r;
 }
 
+// What two choices may be off by, together.  Sigmoid: 14 units of 2^-24 (its argument's rounding, one exponential, one
+// addition, one reciprocal, of values up to 1, twice); softmax: up to 60 (the rounding of logit - top scaled by the
+// score, the sum's own error, twice); additions half a unit in the last place each come on top.  Without a bias the
+// logits themselves are compared.
+__device__ __forceinline__ float choice_error(const Args& a) {
+  return a.bias == nullptr ? 0.f : (a.sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18));
+}
+
 // How groups lie in the lanes: none, whole lanes (a power of two of them) per group, or anyhow.
 enum Groups { kNoGroups = 0, kLaneGroups = 1, kAnyGroups = 2 };
+
+// Weights of a token's picks (lane r holds pick r), and the result.  Renormalised weights are ratios of scores: they are
+// formed relative to the largest pick, so that picks far below the row's largest logit (a bias or a group can choose
+// them) keep their ratios.
+__device__ __forceinline__ void write_weights(const Args& a, int64_t token, const Picks& p, float top, float total, bool spoilt) {
+  const int lane = threadIdx.x & 31;
+  const bool sigmoid = a.sigmoid != 0, has_pick = lane < a.top_k, live = has_pick && p.logit > -INFINITY;
+  float w = 0.f;
+  if (a.renormalize) {
+    const float best = redux_max_nan(live ? p.logit : -INFINITY);
+    if (!sigmoid) {
+      w = live ? expf(p.logit - best) : 0.f;
+    } else {
+      // relative to the best pick's exp(best) where that is negative
+      const float t = expf(-fabsf(p.logit));
+      float numerator = p.logit < 0.f ? t : 1.f;
+      if (best < 0.f) numerator = expf(p.logit - best);
+      w = live ? __fdividef(numerator, 1.f + t) : 0.f;
+    }
+    const float sum = warp_total(w);
+    if (live) w = __fdividef(w, sum);
+  } else if (live) {
+    w = sigmoid ? sigmoid_of(p.logit) : __fdividef(expf(p.logit - top), total);
+  }
+  w = spoilt ? NAN : w * a.scale;
+  if (has_pick) {
+    a.weights[token * a.top_k + lane] = w;
+    a.chosen[token * a.top_k + lane] = p.expert;
+  }
+}
+
+// One token, a warp.  b: the lane's biases (0 without one).
+template <typename T, int VPL, int GROUPS>
+__device__ __forceinline__ void route_token(const Args& a, int64_t token, const float (&b)[VPL], float* my_choices) {
+  constexpr int kIndexBits = 5 + log2_of(VPL), kValueBits = kIndexBits <= 9 ? 23 : 32 - kIndexBits;
+  constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
+  const int lane = threadIdx.x & 31;
+  const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr;
+  const bool by_scores = GROUPS != kNoGroups && a.group_top > 1;  // group scores are sums of scores
+  const float base = choice_error(a);
+  const T* row = static_cast<const T*>(a.logits) + token * a.ld;
+  float c[VPL];  // logits, then choices
+  load_row<T, VPL>(a, row, lane, c);
+  float top = 0.f, total = 0.f, inv_total = 0.f;
+  float hi = c[0];  // a lane's best choice
+#pragma unroll
+  for (int j = 1; j < VPL; ++j) hi = max_nan(hi, c[j]);
+  // A NaN (or, under softmax, an infinite logit) spoils the row's scores: its weights come out as NaN.
+  bool spoilt = false;
+  if (!sigmoid) {
+    top = redux_max_nan(hi);
+    spoilt = top == INFINITY;
+    if (biased || by_scores || !a.renormalize) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) total += exp2_fast(kLog2e * (c[j] - top));
+      total = warp_total(total);
+      inv_total = reciprocal_fast(total);
+    }
+  }
+  if (biased) {
+    float low = c[0];
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) low = fminf(low, c[j]);
+    float choice[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) choice[j] = score_fast(c[j], sigmoid, top, inv_total) + b[j];
+    if (low == -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) choice[j] = c[j] == -INFINITY ? -INFINITY : choice[j];
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) c[j] = choice[j], hi = j == 0 ? c[0] : max_nan(hi, c[j]);
+  }
+  spoilt = __any_sync(kAll, spoilt || hi != hi);
+  bool slow = spoilt;  // decided by choose_exactly
+
+  bool alive = hi > -INFINITY;  // this lane has experts to pick
+  if constexpr (GROUPS != kNoGroups) {
+    // the two best choices of the group that this lane looks through: its own experts' group, or (any layout) one
+    // that 2^lanes_log lanes share
+    const int lanes = 1 << a.lanes_log, group = lane >> a.lanes_log;
+    const bool is_group = group < a.num_groups;
+    float m1 = -INFINITY, m2 = -INFINITY;
+    if constexpr (GROUPS == kLaneGroups) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) m2 = fmaxf(m2, fminf(m1, c[j])), m1 = fmaxf(m1, c[j]);
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) my_choices[lane * VPL + j] = c[j];
+      __syncwarp();
+      if (is_group) {
+        for (int i = lane & (lanes - 1); i < a.group_size; i += lanes) {
+          const float v = my_choices[group * a.group_size + i];
+          m2 = fmaxf(m2, fminf(m1, v));
+          m1 = fmaxf(m1, v);
+        }
+      }
+    }
+    for (int o = 1; o < lanes; o <<= 1) {
+      const float o1 = __shfl_xor_sync(kAll, m1, o), o2 = __shfl_xor_sync(kAll, m2, o);
+      m2 = fmaxf(fmaxf(m2, o2), fminf(m1, o1));
+      m1 = fmaxf(m1, o1);
+    }
+    const bool convert = by_scores && !biased;
+    float s = m1;
+    if (convert && m1 > -INFINITY) s = score_fast(m1, sigmoid, top, inv_total);
+    if (by_scores && m2 > -INFINITY) s += convert ? score_fast(m2, sigmoid, top, inv_total) : m2;
+    // a group's rank: its score's key with the group, counted down, in the last bits
+    const uint32_t s_key = is_group ? (key_of(s) & ~a.group_low) | (a.group_low - uint32_t(group)) : 0u;
+    int before = 0;
+#pragma unroll 4
+    for (int g = 0; g < a.num_groups; ++g) before += __shfl_sync(kAll, s_key, g << a.lanes_log) > s_key;
+    bool stays = is_group && before < a.top_groups;
+    if (a.top_groups < a.num_groups) {
+      const float last = redux_min(stays ? s : INFINITY), first = redux_max_nan(is_group && !stays ? s : -INFINITY);
+      // sums of two are off by twice as much, scores of logits by a softmax's margin at most, and the key's last bits
+      // are (group_low + 1) 2^-23 of a score; 16-bit logits lose nothing to them
+      const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
+      const bool exact = error == 0.f && sizeof(T) == 2;
+      const float slack = 2.f * error + fabsf(last) * (float(a.group_low + 3) * (1.f / (1 << 22))) + 1e-36f;
+      if (!exact && first > -INFINITY && last - first <= slack && !spoilt)
+        stays = refine_groups<T>(a, row, top, group, is_group && s > last + slack, is_group && s >= first - slack && s <= last + slack);
+    }
+    if constexpr (GROUPS == kLaneGroups) {
+      alive = alive && stays;
+      if (!alive) hi = -INFINITY;
+    } else {
+      const unsigned kept = __ballot_sync(kAll, stays);
+      hi = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const uint32_t g = (uint32_t(lane * VPL + j) * a.group_inv) >> 20;
+        if (!((kept >> ((g << a.lanes_log) & 31u)) & 1u)) c[j] = -INFINITY;
+        hi = max_nan(hi, c[j]);
+      }
+      alive = hi > -INFINITY;
+    }
+  }
+
+  // [lo, hi]: what the picks lie in
+  float lo = redux_min(alive ? hi : INFINITY);
+  hi = redux_max_nan(hi);
+  if (__popc(__ballot_sync(kAll, alive)) <= a.top_k) {  // too few lanes: the smallest live choice bounds the picks
+    lo = INFINITY;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) lo = c[j] > -INFINITY ? fminf(lo, c[j]) : lo;
+    lo = redux_min(alive ? lo : INFINITY);
+  }
+  const float range = hi - lo;
+  slow |= !(range < 1e30f);
+  const float scale = float((1 << kValueBits) - 600) * reciprocal_fast(fmaxf(range, 1e-30f));
+  // value 0: below lo, masked or dropped; 1 and up: in the range.  Added to 2^23 it is the sum's last 23 bits, and
+  // what 2^23 itself would leave in the key goes with the index's constant.
+  uint32_t key[VPL], m1 = 0, m2 = 0;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    const float q = fmaxf(fmaf(c[j] - lo, scale, 8388609.f), 8388608.f);
+    key[j] = (__float_as_uint(q) << kIndexBits) + (kIndexMask - uint32_t(lane * VPL + j) - (0x4b000000u << kIndexBits));
+    m2 = max(m2, min(m1, key[j]));
+    m1 = max(m1, key[j]);
+  }
+  if (!alive) m1 = 0;
+  uint32_t pick = 0, left = 0;
+  for (int r = 0; r <= a.top_k; ++r) {  // one more, to compare the last pick with what it left behind
+    left = __reduce_max_sync(kAll, m1);
+    if (lane == r) pick = left;
+    const bool mine = m1 == left;
+    m1 = mine ? m2 : m1;
+    m2 = mine ? 0 : m2;
+    if (mine && m1 == 0) {  // both given up
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) m1 = key[j] < left ? max(m1, key[j]) : m1;
+    }
+  }
+
+  const bool has_pick = lane < a.top_k;
+  slow = __any_sync(kAll, slow || (has_pick && (pick >> kIndexBits) == 0));
+  Picks p{int(kIndexMask - (pick & kIndexMask)), -INFINITY};
+  if (!slow) {
+    if (has_pick) p.logit = float(row[p.expert]);
+    uint32_t next = __shfl_down_sync(kAll, pick, 1);
+    if (lane == a.top_k - 1) next = left;
+    // in units of the keys' values: the choices' error, and two for the values' own rounding
+    const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 2.f);
+    bool close = has_pick && (next >> kIndexBits) != 0 && float((pick >> kIndexBits) - (next >> kIndexBits)) <= margin;
+    if (__any_sync(kAll, close)) {
+      if (close) {  // equal inputs are a tie whatever the precision
+        const int e = int(kIndexMask - (next & kIndexMask));
+        const float bias = biased ? a.bias[p.expert] : 0.f, next_bias = biased ? a.bias[e] : 0.f;
+        close = !(p.logit == float(row[e]) && bias == next_bias);
+      }
+      const unsigned pairs = __ballot_sync(kAll, close);
+      if (pairs != 0) {
+        int count = a.top_k;
+        if ((pairs >> (a.top_k - 1)) & 1u) {  // the last pick and the one left behind: that one takes part too
+          const uint32_t beyond = __reduce_max_sync(kAll, m1);
+          count = a.top_k + 1;
+          slow = count > 32 || ((beyond >> kIndexBits) != 0 && float((left >> kIndexBits) - (beyond >> kIndexBits)) <= margin);
+          if (lane == a.top_k) p.expert = int(kIndexMask - (left & kIndexMask)), p.logit = float(row[p.expert]);
+        }
+        if (!slow) p = refine_picks<T>(a, row, top, p, count);
+      }
+    }
+  }
+  if (slow) p = choose_exactly<T, VPL>(a, row, lane);
+
+  write_weights(a, token, p, top, total, spoilt);
+}
+
+template <int VPL>
+__device__ __forceinline__ void load_bias(const Args& a, float (&b)[VPL]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) b[j] = (a.bias != nullptr && lane * VPL + j < a.experts) ? a.bias[lane * VPL + j] : 0.f;
+}
 
 // CTAs per SM (the exact form, a call that few rows make, would otherwise set the registers and with them the occupancy);
 // the grid is that many and every warp takes its tokens in turn, so all of them end within a token of each other.
@@ -322,84 +547,162 @@ template <int VPL> constexpr int kResident = VPL <= 8 ? 4 : (VPL == 16 ? 2 : 1);
 template <typename T, int VPL, int GROUPS>
 __global__ void __launch_bounds__(kWarps * 32, kResident<VPL>)
 route_experts_kernel(const __grid_constant__ Args a) {
-  constexpr int kIndexBits = 5 + log2_of(VPL), kValueBits = kIndexBits <= 9 ? 23 : 32 - kIndexBits;
-  constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
   __shared__ float shared_choices[GROUPS == kAnyGroups ? kWarps : 1][GROUPS == kAnyGroups ? 32 * VPL : 1];
-  float* my_choices = shared_choices[GROUPS == kAnyGroups ? threadIdx.x >> 5 : 0];
-  const int lane = threadIdx.x & 31;
-  const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr;
-  const bool by_scores = GROUPS != kNoGroups && a.group_top > 1;  // group scores are sums of scores
-  // What two choices may be off by, together.  Sigmoid: 14 units of 2^-24 (its argument's rounding, one exponential,
-  // one addition, one reciprocal, of values up to 1, twice); softmax: up to 60 (the rounding of logit - top scaled by
-  // the score, the sum's own error, twice); additions half a unit in the last place each.  Without a bias the logits
-  // themselves are compared.
-  const float base = !biased ? 0.f : (sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18));
-
   float b[VPL];
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) b[j] = (biased && lane * VPL + j < a.experts) ? a.bias[lane * VPL + j] : 0.f;
-
+  load_bias<VPL>(a, b);
   const int64_t step = int64_t(gridDim.x) * kWarps;
-  for (int64_t token = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); token < a.tokens; token += step) {
-    const T* row = static_cast<const T*>(a.logits) + token * a.ld;
-    float c[VPL];  // logits, then choices
-    load_row<T, VPL>(a, row, lane, c);
-    float top = 0.f, total = 0.f, inv_total = 0.f;
-    float hi = c[0];  // a lane's best choice
+  for (int64_t token = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); token < a.tokens; token += step)
+    route_token<T, VPL, GROUPS>(a, token, b, shared_choices[GROUPS == kAnyGroups ? threadIdx.x >> 5 : 0]);
+}
+
+// ------------------------------------------------------------------ many tokens
+// Four tokens per warp, eight lanes each: what a warp does once per round, group and row then serves four tokens.  A
+// lane holds up to 32 neighbouring experts (staged through shared memory, so that the loads are coalesced and the next
+// tokens' rows are on their way meanwhile) and keeps its four best keys.  The range of the keys starts at the smallest
+// of the lanes' second-best choices where that leaves enough experts in it.  Tokens with near ties among their picks have
+// these compared in 64 bits afterwards, by the whole warp; a token with anything else unsure goes through route_token.  65536 tokens x 256
+// experts, top 8: 43 us in groups (top 4 of 8, biased sigmoid) against 61 with a warp per token, 31 against 38 by softmax;
+// 128 experts in bf16 21 against 34.  In smaller batches the longer work per warp shows as latency: 8192 tokens in groups
+// 13 against 12 us, by softmax 6.3 against 7.0; hence the bounds in launch_many.
+constexpr int kManyWarps = 4;
+constexpr int kManyMaxPicks = 8;
+
+__device__ __forceinline__ float eight_max_nan(float v) {
 #pragma unroll
-    for (int j = 1; j < VPL; ++j) hi = max_nan(hi, c[j]);
-    // A NaN (or, under softmax, an infinite logit) spoils the row's scores: its weights come out as NaN.
-    bool spoilt = false;
+  for (int o = 1; o < 8; o <<= 1) v = max_nan(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+__device__ __forceinline__ float eight_min(float v) {
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) v = fminf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+__device__ __forceinline__ float eight_sum(float v) {
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+__device__ __forceinline__ uint32_t eight_max(uint32_t v) {
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+
+template <typename T, int GROUPS>
+__device__ __noinline__ void route_token_apart(const Args& a, int64_t token, float* scratch) {
+  float b[8];
+  load_bias<8>(a, b);
+  route_token<T, 8, GROUPS>(a, token, b, scratch);
+}
+
+template <typename T>
+__device__ __noinline__ void refine_apart(const Args& a, int64_t token, float top, float total, Picks p, int count) {
+  p = refine_picks<T>(a, static_cast<const T*>(a.logits) + token * a.ld, top, p, count);
+  write_weights(a, token, p, top, total, false);
+}
+
+template <typename T, int VPL, bool GROUPED>
+__global__ void __launch_bounds__(kManyWarps * 32, VPL <= 16 ? 6 : 4)
+route_many_kernel(const __grid_constant__ Args a) {
+  constexpr int kLaneBytes = VPL * int(sizeof(T)) + 16;  // the pad spreads eight lanes' 16-byte reads over the banks
+  constexpr int kRowBytes = 8 * kLaneBytes, kChunks = VPL * int(sizeof(T)) / 16;  // 16-byte chunks of a lane
+  constexpr int kIndexBits = VPL <= 16 ? 7 : 8, kValueBits = 23;
+  constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
+  __shared__ __align__(16) uint8_t staged[kManyWarps][2][4 * kRowBytes];
+  __shared__ __align__(16) float shared_bias[8 * (VPL + 4)];
+  __shared__ float scratch[GROUPED ? kManyWarps : 1][GROUPED ? 256 : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane >> 3, l8 = lane & 7;
+  const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr, by_scores = GROUPED && a.group_top > 1;
+  const float base = choice_error(a);
+  for (int e = threadIdx.x; e < 8 * VPL; e += kManyWarps * 32)
+    shared_bias[e / VPL * (VPL + 4) + e % VPL] = (biased && e < a.experts) ? a.bias[e] : 0.f;
+  __syncthreads();
+
+  const int chunks = a.experts * int(sizeof(T)) / 16;  // of a row
+  auto fetch = [&](int64_t first, int buf) {
+    const int64_t token = first + part < a.tokens ? first + part : a.tokens - 1;
+    const uint8_t* src = static_cast<const uint8_t*>(a.logits) + token * a.ld * int64_t(sizeof(T));
+    uint8_t* dst = staged[warp][buf] + part * kRowBytes;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int q = i * 8 + l8;
+      if (q < chunks)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                     ::"r"(uint32_t(__cvta_generic_to_shared(dst + q / kChunks * kLaneBytes + q % kChunks * 16))), "l"(src + q * 16) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  const int64_t step = int64_t(gridDim.x) * kManyWarps * 4;
+  int64_t first = (int64_t(blockIdx.x) * kManyWarps + warp) * 4;
+  int buf = 0;
+  if (first < a.tokens) fetch(first, 0);
+  for (; first < a.tokens; first += step, buf ^= 1) {
+    if (first + step < a.tokens) fetch(first + step, buf ^ 1);
+    else asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint8_t* rows = staged[warp][buf] + part * kRowBytes;
+    const int64_t token = first + part;
+    bool unsure = false;  // goes through route_token
+
+    float c[VPL];  // logits, then choices
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(rows + l8 * kLaneBytes + i * 16);
+      const T* t = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int j = 0; j < 16 / int(sizeof(T)); ++j) c[i * (16 / int(sizeof(T))) + j] = float(t[j]);
+    }
+    if ((l8 + 1) * VPL > a.experts) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) c[j] = l8 * VPL + j < a.experts ? c[j] : -INFINITY;
+    }
+    float top = 0.f, total = 0.f, inv_total = 0.f;
     if (!sigmoid) {
-      top = redux_max_nan(hi);
-      spoilt = top == INFINITY;
+      top = c[0];
+#pragma unroll
+      for (int j = 1; j < VPL; ++j) top = max_nan(top, c[j]);
+      top = eight_max_nan(top);
       if (biased || by_scores || !a.renormalize) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) total += exp2_fast(kLog2e * (c[j] - top));
-        total = warp_total(total);
+        total = eight_sum(total);
         inv_total = reciprocal_fast(total);
       }
+      unsure = !(top > -INFINITY && top < INFINITY);
     }
     if (biased) {
       float low = c[0];
 #pragma unroll
       for (int j = 1; j < VPL; ++j) low = fminf(low, c[j]);
-      float choice[VPL];
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) choice[j] = score_fast(c[j], sigmoid, top, inv_total) + b[j];
+      const float4* bias = reinterpret_cast<const float4*>(shared_bias + l8 * (VPL + 4));
       if (low == -INFINITY) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) choice[j] = c[j] == -INFINITY ? -INFINITY : choice[j];
-      }
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) c[j] = choice[j], hi = j == 0 ? c[0] : max_nan(hi, c[j]);
-    }
-    spoilt = __any_sync(kAll, spoilt || hi != hi);
-    bool slow = spoilt;  // decided by choose_exactly
-
-    bool alive = hi > -INFINITY;  // this lane has experts to pick
-    if constexpr (GROUPS != kNoGroups) {
-      // the two best choices of the group that this lane looks through: its own experts' group, or (any layout) one
-      // that 2^lanes_log lanes share
-      const int lanes = 1 << a.lanes_log, group = lane >> a.lanes_log;
-      const bool is_group = group < a.num_groups;
-      float m1 = -INFINITY, m2 = -INFINITY;
-      if constexpr (GROUPS == kLaneGroups) {
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) m2 = fmaxf(m2, fminf(m1, c[j])), m1 = fmaxf(m1, c[j]);
+        for (int j = 0; j < VPL; ++j)
+          c[j] = c[j] == -INFINITY ? -INFINITY : score_fast(c[j], sigmoid, top, inv_total) + reinterpret_cast<const float*>(bias)[j];
       } else {
-        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) my_choices[lane * VPL + j] = c[j];
-        __syncwarp();
-        if (is_group) {
-          for (int i = lane & (lanes - 1); i < a.group_size; i += lanes) {
-            const float v = my_choices[group * a.group_size + i];
-            m2 = fmaxf(m2, fminf(m1, v));
-            m1 = fmaxf(m1, v);
-          }
+        for (int j = 0; j < VPL / 4; ++j) {
+          const float4 v = bias[j];
+          c[4 * j] = score_fast(c[4 * j], sigmoid, top, inv_total) + v.x;
+          c[4 * j + 1] = score_fast(c[4 * j + 1], sigmoid, top, inv_total) + v.y;
+          c[4 * j + 2] = score_fast(c[4 * j + 2], sigmoid, top, inv_total) + v.z;
+          c[4 * j + 3] = score_fast(c[4 * j + 3], sigmoid, top, inv_total) + v.w;
         }
       }
+    }
+    // the lane's two best choices (a NaN takes the first place)
+    float hi = c[0], second = -INFINITY;
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) second = fmaxf(second, fminf(hi, c[j])), hi = max_nan(hi, c[j]);
+    const float best = eight_max_nan(hi);
+    unsure |= !(best < INFINITY);  // a NaN, an infinite choice
+    bool alive = hi > -INFINITY;
+    if constexpr (GROUPED) {
+      const int lanes = 1 << a.many_lanes_log, group = l8 >> a.many_lanes_log;
+      const bool is_group = group < a.num_groups;
+      float m1 = hi, m2 = second;
       for (int o = 1; o < lanes; o <<= 1) {
         const float o1 = __shfl_xor_sync(kAll, m1, o), o2 = __shfl_xor_sync(kAll, m2, o);
         m2 = fmaxf(fmaxf(m2, o2), fminf(m1, o1));
@@ -409,131 +712,158 @@ route_experts_kernel(const __grid_constant__ Args a) {
       float s = m1;
       if (convert && m1 > -INFINITY) s = score_fast(m1, sigmoid, top, inv_total);
       if (by_scores && m2 > -INFINITY) s += convert ? score_fast(m2, sigmoid, top, inv_total) : m2;
-      // a group's rank: its score's key with the group, counted down, in the last bits
-      const uint32_t s_key = is_group ? (key_of(s) & ~a.group_low) | (a.group_low - uint32_t(group)) : 0u;
+      const uint32_t s_key = is_group ? (key_of(s) & ~7u) | uint32_t(7 - group) : 0u;
       int before = 0;
-#pragma unroll 4
-      for (int g = 0; g < a.num_groups; ++g) before += __shfl_sync(kAll, s_key, g << a.lanes_log) > s_key;
-      bool stays = is_group && before < a.top_groups;
-      if (a.top_groups < a.num_groups) {
-        const float last = redux_min(stays ? s : INFINITY), first = redux_max_nan(is_group && !stays ? s : -INFINITY);
-        // sums of two are off by twice as much, scores of logits by a softmax's margin at most, and the key's last bits
-        // are (group_low + 1) 2^-23 of a score; 16-bit logits lose nothing to them
-        const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
-        const bool exact = error == 0.f && sizeof(T) == 2;
-        const float slack = 2.f * error + fabsf(last) * (float(a.group_low + 3) * (1.f / (1 << 22))) + 1e-36f;
-        if (!exact && first > -INFINITY && last - first <= slack && !spoilt)
-          stays = refine_groups<T>(a, row, top, group, is_group && s > last + slack, is_group && s >= first - slack && s <= last + slack);
-      }
-      if constexpr (GROUPS == kLaneGroups) {
-        alive = alive && stays;
-        if (!alive) hi = -INFINITY;
-      } else {
-        const unsigned kept = __ballot_sync(kAll, stays);
-        hi = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-          const uint32_t g = (uint32_t(lane * VPL + j) * a.group_inv) >> 20;
-          if (!((kept >> ((g << a.lanes_log) & 31u)) & 1u)) c[j] = -INFINITY;
-          hi = max_nan(hi, c[j]);
-        }
-        alive = hi > -INFINITY;
+      for (int g = 0; g < 8; ++g)
+        if (g < a.num_groups) before += __shfl_sync(kAll, s_key, (lane & 24) + (g << a.many_lanes_log)) > s_key;
+      const bool stays = is_group && before < a.top_groups;
+      if (a.top_groups < a.num_groups) {
+        const float last = eight_min(stays ? s : INFINITY), next = eight_max_nan(is_group && !stays ? s : -INFINITY);
+        // (as in route_token, with three bits of a score's key taken by the group)
+        const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
+        const float slack = 2.f * error + fabsf(last) * (10.f / (1 << 22)) + 1e-36f;
+        unsure |= !(error == 0.f && sizeof(T) == 2) && next > -INFINITY && last - next <= slack;
       }
+      alive = alive && stays;
     }
 
-    // [lo, hi]: what the picks lie in
-    float lo = redux_min(alive ? hi : INFINITY);
-    hi = redux_max_nan(hi);
-    if (__popc(__ballot_sync(kAll, alive)) <= a.top_k) {  // too few lanes: the smallest live choice bounds the picks
+    // [lo, hi]: the lanes' second-best choices leave two experts per live lane in it
+    float lo = eight_min(alive ? second : INFINITY);
+    const int lanes_alive = __popc((__ballot_sync(kAll, alive) >> (lane & 24)) & 255u);
+    if (2 * lanes_alive < a.top_k || !(lo > -INFINITY)) {
       lo = INFINITY;
 #pragma unroll
       for (int j = 0; j < VPL; ++j) lo = c[j] > -INFINITY ? fminf(lo, c[j]) : lo;
-      lo = redux_min(alive ? lo : INFINITY);
+      if (!alive) lo = INFINITY;
     }
+    lo = eight_min(lo);
+    hi = eight_max_nan(alive ? hi : -INFINITY);
+    lo -= 0.125f * (hi - lo);  // room below, so that what is left behind is not mistaken for a neighbour of the last pick
     const float range = hi - lo;
-    slow |= !(range < 1e30f);
+    unsure |= !(range < 1e30f);
     const float scale = float((1 << kValueBits) - 600) * reciprocal_fast(fmaxf(range, 1e-30f));
-    // value 0: below lo, masked or dropped; 1 and up: in the range.  Added to 2^23 it is the sum's last 23 bits, and
-    // what 2^23 itself would leave in the key goes with the index's constant.
-    uint32_t key[VPL], m1 = 0, m2 = 0;
+    uint32_t key[VPL], m1 = 0, m2 = 0, m3 = 0, m4 = 0;
+    const uint32_t index = kIndexMask - uint32_t(l8 * VPL) - (0x4b000000u << kIndexBits);
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
       const float q = fmaxf(fmaf(c[j] - lo, scale, 8388609.f), 8388608.f);
-      key[j] = (__float_as_uint(q) << kIndexBits) + (kIndexMask - uint32_t(lane * VPL + j) - (0x4b000000u << kIndexBits));
+      key[j] = (__float_as_uint(q) << kIndexBits) + (index - uint32_t(j));
+      m4 = max(m4, min(m3, key[j]));
+      m3 = max(m3, min(m2, key[j]));
       m2 = max(m2, min(m1, key[j]));
       m1 = max(m1, key[j]);
     }
-    if (!alive) m1 = 0;
+    if (!alive) m1 = m2 = m3 = m4 = 0;
     uint32_t pick = 0, left = 0;
-    for (int r = 0; r <= a.top_k; ++r) {  // one more, to compare the last pick with what it left behind
-      left = __reduce_max_sync(kAll, m1);
-      if (lane == r) pick = left;
-      const bool mine = m1 == left;
-      m1 = mine ? m2 : m1;
-      m2 = mine ? 0 : m2;
-      if (mine && m1 == 0) {  // both given up
+    for (int r = 0; r <= a.top_k; ++r) {
+      left = eight_max(m1);
+      if (l8 == r) pick = left;
+      const bool mine = m1 == left && left != 0;
+      if (mine) m1 = m2, m2 = m3, m3 = m4, m4 = 0;
+      if (mine && m1 == 0) {  // all four given up
 #pragma unroll
         for (int j = 0; j < VPL; ++j) m1 = key[j] < left ? max(m1, key[j]) : m1;
       }
     }
 
-    const bool has_pick = lane < a.top_k;
-    slow = __any_sync(kAll, slow || (has_pick && (pick >> kIndexBits) == 0));
-    Picks p{int(kIndexMask - (pick & kIndexMask)), -INFINITY};
-    if (!slow) {
-      if (has_pick) p.logit = float(row[p.expert]);
-      uint32_t next = __shfl_down_sync(kAll, pick, 1);
-      if (lane == a.top_k - 1) next = left;
-      // in units of the keys' values: the choices' error, and two for the values' own rounding
-      const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 2.f);
-      bool close = has_pick && (next >> kIndexBits) != 0 && float((pick >> kIndexBits) - (next >> kIndexBits)) <= margin;
-      if (__any_sync(kAll, close)) {
-        if (close) {  // equal inputs are a tie whatever the precision
-          const int e = int(kIndexMask - (next & kIndexMask));
-          const float bias = biased ? a.bias[p.expert] : 0.f, next_bias = biased ? a.bias[e] : 0.f;
-          close = !(p.logit == float(row[e]) && bias == next_bias);
-        }
-        const unsigned pairs = __ballot_sync(kAll, close);
-        if (pairs != 0) {
-          int count = a.top_k;
-          if ((pairs >> (a.top_k - 1)) & 1u) {  // the last pick and the one left behind: that one takes part too
-            const uint32_t beyond = __reduce_max_sync(kAll, m1);
-            count = a.top_k + 1;
-            slow = count > 32 || ((beyond >> kIndexBits) != 0 && float((left >> kIndexBits) - (beyond >> kIndexBits)) <= margin);
-            if (lane == a.top_k) p.expert = int(kIndexMask - (left & kIndexMask)), p.logit = float(row[p.expert]);
-          }
-          if (!slow) p = refine_picks<T>(a, row, top, p, count);
-        }
+    const bool has_pick = l8 < a.top_k;
+    uint32_t next = __shfl_down_sync(kAll, pick, 1);
+    if (l8 == a.top_k - 1) next = left;
+    const uint32_t value = pick >> kIndexBits, next_value = next >> kIndexBits;
+    const int expert = min(int(kIndexMask - (pick & kIndexMask)), a.experts - 1);
+    auto logit_of = [&](int e) {
+      return float(*reinterpret_cast<const T*>(rows + e / VPL * kLaneBytes + e % VPL * int(sizeof(T))));
+    };
+    const float logit = has_pick ? logit_of(expert) : -INFINITY;
+    // one more than in route_token: what was left behind may lie below lo
+    const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 3.f);
+    bool close = has_pick && next != 0 && float(value - next_value) <= margin;
+    if (__any_sync(kAll, close)) {
+      if (close) {  // equal inputs are a tie whatever the precision
+        const int e = min(int(kIndexMask - (next & kIndexMask)), a.experts - 1);
+        close = !(next_value != 0 && logit == logit_of(e) && (!biased || a.bias[expert] == a.bias[e]));
       }
     }
-    if (slow) p = choose_exactly<T, VPL>(a, row, lane);
+    unsure |= has_pick && value == 0;
+    const unsigned unsure_lanes = __ballot_sync(kAll, unsure), close_lanes = __ballot_sync(kAll, close);
+    const bool done = (((unsure_lanes | close_lanes) >> (lane & 24)) & 255u) == 0;
 
-    // Weights.  Renormalised ones are ratios of scores: they are formed relative to the largest pick, so that picks
-    // far below the row's largest logit (a bias or a group can choose them) keep their ratios.
-    const bool live = has_pick && p.logit > -INFINITY;
+    // weights, as in write_weights
     float w = 0.f;
     if (a.renormalize) {
-      const float best = redux_max_nan(live ? p.logit : -INFINITY);
+      const float most = eight_max_nan(logit);
       if (!sigmoid) {
-        w = live ? expf(p.logit - best) : 0.f;
+        w = has_pick ? expf(logit - most) : 0.f;
       } else {
-        // relative to the best pick's exp(best) where that is negative
-        const float t = expf(-fabsf(p.logit));
-        float numerator = p.logit < 0.f ? t : 1.f;
-        if (best < 0.f) numerator = expf(p.logit - best);
-        w = live ? __fdividef(numerator, 1.f + t) : 0.f;
+        const float t = expf(-fabsf(logit));
+        float numerator = logit < 0.f ? t : 1.f;
+        if (most < 0.f) numerator = expf(logit - most);
+        w = has_pick ? __fdividef(numerator, 1.f + t) : 0.f;
       }
-      const float sum = warp_total(w);
-      if (live) w = __fdividef(w, sum);
-    } else if (live) {
-      w = sigmoid ? sigmoid_of(p.logit) : __fdividef(expf(p.logit - top), total);
+      w = __fdividef(w, eight_sum(w));
+    } else {
+      w = sigmoid ? sigmoid_of(logit) : __fdividef(expf(logit - top), total);
     }
-    w = spoilt ? NAN : w * a.scale;
-    if (has_pick) {
-      a.weights[token * a.top_k + lane] = w;
-      a.chosen[token * a.top_k + lane] = p.expert;
+    if (has_pick && done && token < a.tokens) {
+      a.weights[token * a.top_k + l8] = w * a.scale;
+      a.chosen[token * a.top_k + l8] = expert;
     }
+    __syncwarp();
+    if ((unsure_lanes | close_lanes) != 0) {
+      const uint32_t beyond = eight_max(m1);
+      // the last pick and the one left behind are close: that one takes part, if it is clear of what comes after it
+      const bool clear = (left >> kIndexBits) != 0 && float((left >> kIndexBits) - (beyond >> kIndexBits)) > margin;
+      unsure = !clear && ((close_lanes >> ((lane & 24) + a.top_k - 1)) & 1u);
+      const unsigned tied = __ballot_sync(kAll, unsure);
+      for (int t = 0; t < 4; ++t) {
+        const unsigned close_t = (close_lanes >> (8 * t)) & 255u;
+        if (first + t >= a.tokens) break;
+        if ((((unsure_lanes | tied) >> (8 * t)) & 255u) != 0) {
+          route_token_apart<T, GROUPED ? kAnyGroups : kNoGroups>(a, first + t, scratch[GROUPED ? warp : 0]);
+        } else if (close_t != 0) {
+          const int source = 8 * t + (lane & 7);
+          Picks p{__shfl_sync(kAll, expert, source), __shfl_sync(kAll, logit, source)};
+          const uint32_t left_t = __shfl_sync(kAll, left, 8 * t);
+          const bool joins = (close_t >> (a.top_k - 1)) & 1u;
+          if (joins && lane == a.top_k) {
+            p.expert = int(kIndexMask - (left_t & kIndexMask));
+            p.logit = float(*reinterpret_cast<const T*>(staged[warp][buf] + t * kRowBytes + p.expert / VPL * kLaneBytes + p.expert % VPL * int(sizeof(T))));
+          }
+          refine_apart<T>(a, first + t, __shfl_sync(kAll, top, 8 * t), __shfl_sync(kAll, total, 8 * t), p, a.top_k + (joins ? 1 : 0));
+        }
+      }
+    }
+    __syncwarp();
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Returns false for what the kernel does not take.
+template <typename T, int VPL>
+bool launch_many_vpl(Args a, cudaStream_t s) {
+  const int lanes = a.group_size / VPL;
+  const bool grouped = a.num_groups > 1;
+  if (grouped && (a.group_size % VPL != 0 || (lanes & (lanes - 1)) != 0)) return false;
+  a.many_lanes_log = 0;
+  while (grouped && (1 << a.many_lanes_log) < lanes) ++a.many_lanes_log;
+  const int64_t blocks = (a.tokens + 4 * kManyWarps - 1) / (4 * kManyWarps), places = (VPL <= 16 ? 6 : 4) * 148;
+  const int grid = int(blocks < places ? blocks : places);
+  if (grouped) route_many_kernel<T, VPL, true><<<grid, kManyWarps * 32, 0, s>>>(a);
+  else route_many_kernel<T, VPL, false><<<grid, kManyWarps * 32, 0, s>>>(a);
+  return true;
+}
+
+template <typename T>
+bool launch_many(const Args& a, cudaStream_t s) {
+  constexpr int kSize = int(sizeof(T));
+  if (a.tokens < (a.num_groups > 1 ? 16384 : 8192) || a.top_k > kManyMaxPicks || a.experts < 32 || a.experts > 256 || (a.experts * kSize) % 16 != 0 ||
+      (a.ld * kSize) % 16 != 0 || reinterpret_cast<uintptr_t>(a.logits) % 16 != 0)
+    return false;
+  if (a.experts <= 64) return launch_many_vpl<T, 8>(a, s);
+  if (a.experts <= 128) return launch_many_vpl<T, 16>(a, s);
+  if (a.experts <= 192) return launch_many_vpl<T, 24>(a, s);
+  return launch_many_vpl<T, 32>(a, s);
 }
 
 template <typename T, int VPL>
@@ -558,6 +888,7 @@ int launch_vpl(Args& a, cudaStream_t s) {
 
 template <typename T>
 int launch(Args& a, cudaStream_t s) {
+  if (launch_many<T>(a, s)) return launch_status();
   if (a.experts <= 32) return launch_vpl<T, 1>(a, s);
   if (a.experts <= 64) return launch_vpl<T, 2>(a, s);
   if (a.experts <= 128) return launch_vpl<T, 4>(a, s);

@@ -108,6 +108,59 @@ def test_ties_go_to_the_lowest_index():
         compare(logits, 8, **kw)
 
 
+MANY = [
+    (32, 2, {}),
+    (64, 6, dict(renormalize=True, bias=True)),
+    (64, 8, dict(scoring="sigmoid", bias=True, num_groups=8, top_groups=4, group_top=2, renormalize=True, scale=2.5)),
+    (96, 4, dict(bias=True)),
+    (128, 8, {}),
+    (128, 8, dict(scoring="sigmoid", num_groups=4, top_groups=2, group_top=2)),
+    (128, 1, dict(num_groups=8, top_groups=1, renormalize=True)),
+    (160, 6, dict(num_groups=8, top_groups=3, scale=16.0)),
+    (192, 8, dict(scoring="sigmoid", bias=True, num_groups=8, top_groups=4, group_top=2)),
+    (200, 5, dict(scoring="sigmoid", renormalize=True)),
+    (256, 8, dict(scoring="sigmoid", bias=True, num_groups=8, top_groups=4, group_top=2, renormalize=True, scale=2.5)),
+    (256, 8, dict(num_groups=2, top_groups=1)),
+    (256, 8, dict(num_groups=8, top_groups=1, group_top=2, bias=True)),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("experts,top_k,kw", MANY)
+def test_many_tokens(experts, top_k, kw, dtype):
+    """Large batches take another form: every token as in a small batch and as in the definition, whatever the row
+    holds (masked experts, the type's lowest value as a mask, ties, NaN, nothing at all)."""
+    tokens = 16403
+    logits, k = make(tokens, experts, dtype, kw, seed=7)
+    g = torch.Generator(device=DEV).manual_seed(experts)
+    logits[100:200][torch.rand(100, experts, generator=g, device=DEV) < 0.6] = -math.inf
+    logits[200:300][torch.rand(100, experts, generator=g, device=DEV) < 0.3] = torch.finfo(dtype).min
+    logits[300:340] = 0.25
+    logits[340:360] = torch.randint(0, 3, (20, experts), generator=g, device=DEV).to(dtype)
+    logits[360, 5], logits[361, 1::2], logits[362] = math.nan, math.nan, -math.inf
+    logits[363, 3] = math.inf
+    logits[364, : experts - 1] = -math.inf
+    logits[365] = torch.finfo(dtype).max
+    logits[400:420] *= 40
+    w, e = hb.route_experts(logits, top_k, **k)
+    # a warp per token, 5000 at a time
+    parts = [hb.route_experts(logits[i : i + 5000], top_k, **k) for i in range(0, tokens, 5000)]
+    we, ee = torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
+    assert torch.equal(e, ee)
+    assert torch.equal(torch.isnan(w), torch.isnan(we))
+    assert ((w - we).abs() <= 2.0**-19 * we.abs() + 1e-38).logical_or(torch.isnan(we)).all()
+    keep = torch.tensor([i for i in range(420) if i not in (360, 361, 363)] + [tokens - 2, tokens - 1], device=DEV)
+    compare(logits[keep], top_k, **k)  # (the small form)
+    rw, re = route(logits[keep], top_k, **k)
+    assert torch.equal(e[keep].cpu(), re)
+    # not contiguous: the same answers from a pitched view, aligned and not
+    wide = torch.full((tokens, experts + 24), math.nan, dtype=dtype, device=DEV)
+    for at in (8, 3):
+        wide[:, at : at + experts] = logits
+        w2, e2 = hb.route_experts(wide[:, at : at + experts], top_k, **k)
+        assert torch.equal(e2, e) and ((w2 - w).abs() <= 2.0**-19 * w.abs() + 1e-38).logical_or(torch.isnan(w)).all()
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 def test_choices_closer_than_fp32_can_tell(scoring):
     """Biases that make pairs of choices meet to within 2^-26: the picks are still those of exact arithmetic."""
