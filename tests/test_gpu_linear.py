@@ -2,6 +2,10 @@
 
 from __future__ import annotations
 
+from pathlib import Path
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -209,6 +213,37 @@ def test_streams_and_graphs_are_independent():
             graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(y, w) for (_, y), w in zip(graphs, want)) and status_ok()
+
+
+FIRST_CALL = """
+import sys; sys.path.insert(0, {root!r})
+import torch
+import helion_b200 as hb
+torch.manual_seed(0)
+cases = []
+for m, n, k in ((1, 256, 512), (100, 8192, 1024), (512, 1024, 4096), (2048, 2048, 512)):
+    x = torch.randn(m, k, device="cuda").to(torch.bfloat16)
+    cases.append((x, (torch.randn(n, k, device="cuda") / k**0.5).to(torch.bfloat16)))
+logits = torch.randn(20000, 64, device="cuda")
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    ys = [hb.linear(x, w, activation="silu") for x, w in cases]
+    few, many = hb.route_experts(logits[:50], 4), hb.route_experts(logits, 4)
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(y, hb.linear(x, w, activation="silu")) for y, (x, w) in zip(ys, cases))
+for got, want in ((few, hb.route_experts(logits[:50], 4)), (many, hb.route_experts(logits, 4))):
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("captured")
+"""
+
+
+def test_first_call_of_a_process_may_be_captured():
+    code = FIRST_CALL.format(root=str(Path(__file__).resolve().parent.parent))
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
 
 
 def test_registered_operator_and_inference_only():
