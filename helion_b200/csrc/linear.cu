@@ -210,6 +210,12 @@ __device__ __forceinline__ void drain_loads(uint64_t* full_bar, int stages, int 
     while (!mbar_try_wait(smem_u32(&full_bar[it % stages]), (it / stages) & 1) && clock64() - t0 < 20000000) {}
 }
 
+// ... and its MMAs finish: they were committed to `bar`, whose phase this waits for.
+__device__ __forceinline__ void drain_mmas(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - t0 < 20000000) {}
+}
+
 // ------------------------------------------------------------------ streaming kernel
 constexpr int kStreamThreads = 192;
 constexpr int kTileRows = 128;                 // weight rows per tile
@@ -306,8 +312,9 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       }
       __syncwarp();
     }
-    if (ok && elect_one()) tcgen05_commit(smem_u32(done_bar));
+    if (elect_one()) tcgen05_commit(smem_u32(done_bar));
     __syncwarp();
+    if (!ok) drain_mmas(smem_u32(done_bar), 0);
   } else {
     warp_wait(smem_u32(done_bar), 0, abort_flag);
     tcgen05_fence_after();
@@ -637,6 +644,13 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           __syncwarp();
           if (++s == uint32_t(num_stages)) s = 0, phase ^= 1;
         }
+        if (!ok) break;  // (keeps tc, the accumulator of the tile that was given up)
+      }
+      if (!ok) {
+        const uint32_t bar = smem_u32(&tmem_full_bar[tc % kAcc]);
+        if (elect_one()) tcgen05_commit_pair(bar, pair_mask);
+        __syncwarp();
+        drain_mmas(bar, (tc / kAcc) & 1);
       }
     }
   } else {

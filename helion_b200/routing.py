@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
+import functools
 import struct
 
 import torch
@@ -19,13 +20,8 @@ _ARGS = struct.Struct("=11q3if")  # hb200_route_args
 _LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
-           group_top: int) -> None:
-    if router_logits.dim() != 2:
-        raise ValueError("router_logits must be [tokens, experts]")
-    experts = router_logits.shape[1]
-    if router_logits.dtype not in _LOGIT_DTYPES:
-        raise TypeError(f"router_logits must be bfloat16, float16 or float32, got {router_logits.dtype}")
+@functools.lru_cache(maxsize=64)  # a model's settings: looked at once
+def _check_settings(experts: int, top_k: int, scoring: str, num_groups: int, top_groups: int, group_top: int) -> None:
     if not 1 <= experts <= 1024:
         raise ValueError(f"1 to 1024 experts are supported, got {experts}")
     if scoring not in _SCORINGS:
@@ -39,6 +35,16 @@ def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None,
         raise ValueError(f"group_top must be 1 or 2 and at most a group's {size} experts; got {group_top}")
     if not 1 <= top_k <= min(32, top_groups * size):
         raise ValueError(f"top_k must be in 1..{min(32, top_groups * size)}, got {top_k}")
+
+
+def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
+           group_top: int) -> None:
+    if router_logits.dim() != 2:
+        raise ValueError("router_logits must be [tokens, experts]")
+    experts = router_logits.shape[1]
+    if router_logits.dtype not in _LOGIT_DTYPES:
+        raise TypeError(f"router_logits must be bfloat16, float16 or float32, got {router_logits.dtype}")
+    _check_settings(experts, top_k, scoring, num_groups, top_groups, group_top)
     if bias is not None:
         if bias.shape != (experts,):
             raise ValueError(f"bias must be [{experts}], got {tuple(bias.shape)}")

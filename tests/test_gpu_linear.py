@@ -215,6 +215,58 @@ def test_streams_and_graphs_are_independent():
     assert all(torch.equal(y, w) for (_, y), w in zip(graphs, want)) and status_ok()
 
 
+def test_operands_written_by_the_kernel_in_front():
+    """Launches overlap the tail of the kernel in front of them: x, weight, bias and residual that it wrote are seen
+    whole, by this operator and by the package's other overlapping kernel behind it, eagerly and from a graph."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(*shape, generator=g, device=DEV) * std).to(torch.bfloat16)
+
+    x, seed_w = normal(512, 512), normal(512, 512, std=512**-0.5)
+    a8 = (torch.randn(16, 512, generator=g, device=DEV) * 0.05).to(torch.float8_e4m3fn)
+    b8 = [(torch.randn(1024, 512, generator=g, device=DEV) * 0.05).to(torch.float8_e4m3fn) for _ in range(2)]
+    one = torch.ones(1, device=DEV)
+    buf, weight8 = torch.empty_like(x), torch.empty_like(b8[0])
+    c = torch.empty(16, 1024, dtype=torch.bfloat16, device=DEV)
+
+    def chain(sync):
+        out = []
+        wait = torch.cuda.synchronize if sync else (lambda: None)
+        w, r = seed_w, x
+        for step in range(12):
+            m = (512, 3, 96, 40)[step % 4]
+            y = hb.linear(x, w, residual=r, activation="gelu_tanh")  # [512, 512]
+            wait()
+            z = hb.linear(y[:m], y, y[0], residual=r[:m])  # what was just written as x, weight and bias
+            wait()
+            buf.copy_(y)
+            wait()
+            u = hb.linear(z, buf, activation="silu_and_mul")  # the weight copied a moment ago
+            wait()
+            weight8.copy_(b8[step % 2])
+            wait()
+            v = hb.linear(x[:2], buf)
+            wait()
+            hb.scaled_mm(c, a8, weight8.t(), one, one)  # its weight was written before the linear call in front of it
+            wait()
+            out += [y, z, u, v, c.clone()]
+            wait()
+            w, r = (y * 0.05).to(torch.bfloat16), y
+        return out
+
+    want = chain(True)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(False)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and status_ok()
+
+
 FIRST_CALL = """
 import sys; sys.path.insert(0, {root!r})
 import torch
