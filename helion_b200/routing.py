@@ -20,7 +20,6 @@ _ARGS = struct.Struct("=11q3if")  # hb200_route_args
 _LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-@functools.lru_cache(maxsize=64)  # a model's settings: looked at once
 def _check_settings(experts: int, top_k: int, scoring: str, num_groups: int, top_groups: int, group_top: int) -> None:
     if not 1 <= experts <= 1024:
         raise ValueError(f"1 to 1024 experts are supported, got {experts}")
@@ -37,6 +36,9 @@ def _check_settings(experts: int, top_k: int, scoring: str, num_groups: int, top
         raise ValueError(f"top_k must be in 1..{min(32, top_groups * size)}, got {top_k}")
 
 
+_check_settings_once = functools.lru_cache(maxsize=64)(_check_settings)  # a model's settings: looked at once
+
+
 def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int, top_groups: int,
            group_top: int) -> None:
     if router_logits.dim() != 2:
@@ -44,7 +46,9 @@ def _check(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | None,
     experts = router_logits.shape[1]
     if router_logits.dtype not in _LOGIT_DTYPES:
         raise TypeError(f"router_logits must be bfloat16, float16 or float32, got {router_logits.dtype}")
-    _check_settings(experts, top_k, scoring, num_groups, top_groups, group_top)
+    # (under tracing a size may be a symbol, which has no hash)
+    check = _check_settings if torch.compiler.is_compiling() or type(experts) is not int else _check_settings_once
+    check(experts, top_k, scoring, num_groups, top_groups, group_top)
     if bias is not None:
         if bias.shape != (experts,):
             raise ValueError(f"bias must be [{experts}], got {tuple(bias.shape)}")

@@ -405,3 +405,21 @@ def test_moe_block_from_router_to_shared_expert(t):
     assert all(torch.equal(a, b) for a, b in zip(captured, block()))
     torch.cuda.synchronize()
     assert _lib.load().hb200_device_status(1) == 0
+
+
+def test_block_traces_as_one_graph():
+    """Router product, routing and a residual product under torch.compile with changing numbers of tokens."""
+    g = torch.Generator().manual_seed(2)
+    w_r = torch.randn(32, 256, generator=g).to(torch.bfloat16).to(DEV)
+    w = (torch.randn(256, 256, generator=g) / 16).to(torch.bfloat16).to(DEV)
+    routing = hb.Routing(bias=torch.randn(32, generator=g).to(DEV) * 0.1, **ROUTING)
+
+    def block(x):
+        weights, experts = routing(hb.linear(x, w_r, out_dtype=torch.float32), 4)
+        return weights, experts, hb.linear(x, w, activation="silu", residual=x)
+
+    compiled = torch.compile(block, backend="aot_eager", fullgraph=True, dynamic=True)
+    with torch.no_grad():
+        for t in (5, 9, 300):
+            x = torch.randn(t, 256, generator=g).to(torch.bfloat16).to(DEV)
+            assert all(torch.equal(a, b) for a, b in zip(compiled(x), block(x)))
