@@ -11,6 +11,7 @@ import struct
 
 import torch
 from torch import Tensor
+from torch._C import _are_functorch_transforms_active as _in_transform
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import _lib
@@ -151,9 +152,10 @@ def _(x, weight, bias, residual, activation, out_dtype):
 
 
 def _direct(*tensors: Tensor | None) -> bool:
-    """Whether a call can go straight to its kernel: nothing traces, and no subclass or gradient is involved.  The
-    dispatch of a registered operator written in Python costs more host time than a small call's kernel runs."""
-    if torch.compiler.is_compiling() or _get_current_dispatch_mode() is not None:
+    """Whether a call can go straight to its kernel: nothing traces or transforms (the tensors of a ``torch.func``
+    transform look plain but have no address), and no subclass or gradient is involved.  The dispatch of a registered
+    operator written in Python costs more host time than a small call's kernel runs."""
+    if torch.compiler.is_compiling() or _get_current_dispatch_mode() is not None or _in_transform():
         return False
     grad = torch.is_grad_enabled()
     for t in tensors:

@@ -309,3 +309,18 @@ def test_registered_operator_and_inference_only():
         assert torch.equal(hb.linear(a["x"], w, a["bias"]), want)
     with pytest.raises(RuntimeError):
         hb.linear(a["x"], w, a["bias"]).float().sum().backward()
+
+
+def test_function_transforms():
+    """Inside torch.func transforms tensors have no address of their own: the call goes through the registered operator."""
+    a, out = make(6, 64, 128, residual=True)
+    want = call(a, out)
+    one_row = torch.vmap(lambda x, r: hb.linear(x, a["weight"], residual=r))(a["x"], a["residual"])
+    assert torch.equal(one_row, torch.stack([hb.linear(x, a["weight"], residual=r) for x, r in zip(a["x"], a["residual"])]))
+    kept = torch.func.functionalize(lambda r: hb.linear(a["x"], a["weight"], residual=r))(a["residual"])
+    assert torch.equal(kept, want)
+    bias = torch.randn(16, device=DEV)
+    logits = torch.randn(5, 16, device=DEV)
+    for got, plain in zip(torch.func.functionalize(lambda b: hb.route_experts(logits, 3, bias=b))(bias),
+                          hb.route_experts(logits, 3, bias=bias)):
+        assert torch.equal(got, plain)
