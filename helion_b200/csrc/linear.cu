@@ -498,7 +498,8 @@ __device__ __forceinline__ void flush_box(const Args& g, const uint8_t* box, int
   for (int i = 0; i < 32; i += kRowsAtOnce) {
     const int r = i + lane / kCols;
     if (row0 + r < g.m && col + c < g.n)
-      dst[int64_t(row0 + r) * g.ldo + col + c] = *reinterpret_cast<const OutT*>(box + box_chunk(r, c / kPer) + (c % kPer) * sizeof(OutT));
+      dst[int64_t(row0 + r) * g.ldo + col + c] =
+          *reinterpret_cast<const OutT*>(box + box_chunk(r, c / kPer) + (c % kPer) * sizeof(OutT));
   }
 }
 
@@ -970,7 +971,8 @@ PairPlan plan_pair(int64_t m, int64_t weight_rows, int64_t k, int dev, int sms, 
     const int64_t tiles = m_tiles * n_tiles;
     for (int log = 0; log < 3; ++log) {
       if (log > 0 && (num_kb < 4 << log ||
-                      tiles > max_clusters<linear_pair_kernel<__nv_bfloat16, __nv_bfloat16, false, true>>(dev, 0, 2 << log, kPairThreads, kPairSmem)))
+                      tiles > max_clusters<linear_pair_kernel<__nv_bfloat16, __nv_bfloat16, false, true>>(
+                                  dev, 0, 2 << log, kPairThreads, kPairSmem)))
         break;
       const double pairs = sms / 2, busy = double(tiles << log) < pairs ? double(tiles << log) / pairs : 1.0;
       const double waves = log > 0 ? 1.0 : double((tiles + sms / 2 - 1) / (sms / 2));
@@ -1072,7 +1074,8 @@ extern "C" int hb200_linear(const hb200_linear_args* args, void* stream) {
   using namespace hb200;
   using namespace hb200::linear;
   if (!args) return HB200_ERR_INVALID_ARGUMENT;
-  const auto [x, weight, bias, residual, out, m, n, k, ldx, ldw, ldr, ldo, activation, gated, is_bf16, bias_f32, out_f32, reserved] = *args;
+  const auto [x, weight, bias, residual, out, m, n, k, ldx, ldw, ldr, ldo, activation, gated, is_bf16, bias_f32, out_f32,
+              reserved] = *args;
   if (!x || !weight || !out || m <= 0 || n <= 0 || k <= 0 || ldx < k || ldw < k || ldo < n || (residual && ldr < 0))
     return HB200_ERR_INVALID_ARGUMENT;
   if (activation < kNone || activation > kGeluTanh || reserved != 0) return HB200_ERR_INVALID_ARGUMENT;
@@ -1112,7 +1115,8 @@ extern "C" int hb200_linear(const hb200_linear_args* args, void* stream) {
   const PairPlan q = m > 64 ? plan_pair(m, weight_rows, k, dev, sms, &pair_us) : PairPlan{};
   if (m > 64 && pair_us < stream_us(p, double(weight_rows) * double(k) * 2, sms)) {
     if (q.m_tiles * q.n_tiles > 0x7fffffff) return HB200_ERR_UNSUPPORTED;
-    if (!make_map(&tw, weight, weight_rows, k, ldw, q.tile_cols / 2, bf16) || !make_map(&tx, x, m, k, ldx, 128, bf16)) return HB200_ERR_CUDA;
+    if (!make_map(&tw, weight, weight_rows, k, ldw, q.tile_cols / 2, bf16) || !make_map(&tx, x, m, k, ldx, 128, bf16))
+      return HB200_ERR_CUDA;
     if ((n * out_size) % 16 != 0) g.out_vec = 0;  // a TMA store's last 16 bytes of a row are written whole
     if (g.out_vec && !make_out_map(&to, out, m, n, ldo, f32, bf16)) return HB200_ERR_CUDA;
     g.m_tiles = int(q.m_tiles);

@@ -560,9 +560,9 @@ route_experts_kernel(const __grid_constant__ Args a) {
 // lane holds up to 32 neighbouring experts (staged through shared memory, so that the loads are coalesced and the next
 // tokens' rows are on their way meanwhile) and keeps its four best keys.  The range of the keys starts at the smallest
 // of the lanes' second-best choices where that leaves enough experts in it.  Tokens with near ties among their picks have
-// these compared in 64 bits afterwards, by the whole warp; a token with anything else unsure goes through route_token.  65536 tokens x 256
-// experts, top 8: 43 us in groups (top 4 of 8, biased sigmoid) against 61 with a warp per token, 31 against 38 by softmax;
-// 128 experts in bf16 21 against 34.  In smaller batches the longer work per warp shows as latency: 8192 tokens in groups
+// these compared in 64 bits afterwards, by the whole warp; a token with anything else unsure goes through route_token.
+// 65536 tokens x 256 experts, top 8: 43 us in groups (top 4 of 8, biased sigmoid) against 61 with a warp per token, 31
+// against 38 by softmax; 128 experts in bf16 21 against 34.  In smaller batches the longer work per warp shows as latency: 8192 tokens in groups
 // 13 against 12 us, by softmax 6.3 against 7.0; hence the bounds in launch_many.
 constexpr int kManyWarps = 4;
 constexpr int kManyMaxPicks = 8;
@@ -628,7 +628,9 @@ route_many_kernel(const __grid_constant__ Args a) {
       const int q = i * 8 + l8;
       if (q < chunks)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                     ::"r"(uint32_t(__cvta_generic_to_shared(dst + q / kChunks * kLaneBytes + q % kChunks * 16))), "l"(src + q * 16) : "memory");
+                     ::"r"(uint32_t(__cvta_generic_to_shared(dst + q / kChunks * kLaneBytes + q % kChunks * 16))),
+                     "l"(src + q * 16)
+                     : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -828,9 +830,11 @@ route_many_kernel(const __grid_constant__ Args a) {
           const bool joins = (close_t >> (a.top_k - 1)) & 1u;
           if (joins && lane == a.top_k) {
             p.expert = int(kIndexMask - (left_t & kIndexMask));
-            p.logit = float(*reinterpret_cast<const T*>(staged[warp][buf] + t * kRowBytes + p.expert / VPL * kLaneBytes + p.expert % VPL * int(sizeof(T))));
+            p.logit = float(*reinterpret_cast<const T*>(staged[warp][buf] + t * kRowBytes + p.expert / VPL * kLaneBytes +
+                                                        p.expert % VPL * int(sizeof(T))));
           }
-          refine_apart<T>(a, first + t, __shfl_sync(kAll, top, 8 * t), __shfl_sync(kAll, total, 8 * t), p, a.top_k + (joins ? 1 : 0));
+          refine_apart<T>(a, first + t, __shfl_sync(kAll, top, 8 * t), __shfl_sync(kAll, total, 8 * t), p,
+                          a.top_k + (joins ? 1 : 0));
         }
       }
     }
@@ -857,8 +861,8 @@ bool launch_many_vpl(Args a, cudaStream_t s) {
 template <typename T>
 bool launch_many(const Args& a, cudaStream_t s) {
   constexpr int kSize = int(sizeof(T));
-  if (a.tokens < (a.num_groups > 1 ? 16384 : 8192) || a.top_k > kManyMaxPicks || a.experts < 32 || a.experts > 256 || (a.experts * kSize) % 16 != 0 ||
-      (a.ld * kSize) % 16 != 0 || reinterpret_cast<uintptr_t>(a.logits) % 16 != 0)
+  if (a.tokens < (a.num_groups > 1 ? 16384 : 8192) || a.top_k > kManyMaxPicks || a.experts < 32 || a.experts > 256 ||
+      (a.experts * kSize) % 16 != 0 || (a.ld * kSize) % 16 != 0 || reinterpret_cast<uintptr_t>(a.logits) % 16 != 0)
     return false;
   if (a.experts <= 64) return launch_many_vpl<T, 8>(a, s);
   if (a.experts <= 128) return launch_many_vpl<T, 16>(a, s);

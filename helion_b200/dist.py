@@ -541,7 +541,8 @@ def expert_parallel_moe(x: Tensor, router_logits: Tensor, top_k: int, num_expert
     """MoE layer over expert-parallel ranks with the process group's all-to-all as the data plane.
     ``x [T_local, H]`` are this rank's tokens; ``expert_fn`` applies this rank's experts to the rows it receives
     (no routing weight).  Returns bf16 ``[T_local, H]``.  ``router`` and ``combine`` default to the CUDA kernels
-    (``moe.route_top_k``, :func:`combine_rows`; a :class:`~helion_b200.routing.Routing` is a router too); host-logic tests inject tensor-code stand-ins."""
+    (``moe.route_top_k``, :func:`combine_rows`; a :class:`~helion_b200.routing.Routing` is a router too); host-logic
+    tests inject tensor-code stand-ins."""
     if router is None:
         from .moe import route_top_k as router
     if combine is None:

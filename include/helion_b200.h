@@ -457,8 +457,8 @@ int hb200_dense_matmul(const void* a, const void* b, void* c, int64_t m, int64_t
  * (out_f32 != 0).  Pitches in elements; ldr may be 0 (one row for all).  Any M, N >= 1; K % 8 == 0, 16-byte aligned x
  * and weight, ldx % 8 == ldw % 8 == 0 (HB200_ERR_UNSUPPORTED otherwise).  No workspace.  residual may be out itself
  * (same pitch).  The arguments come in a struct (read before the call returns): one pointer instead of eighteen values
- * halves what a foreign-function call costs.  No counterpart in the reference (its examples fuse an epilogue into a matmul through a Python
- * callable). */
+ * halves what a foreign-function call costs.  No counterpart in the reference (its examples fuse an epilogue into a
+ * matmul through a Python callable). */
 typedef struct {
   const void *x, *weight, *bias, *residual;
   void* out;
