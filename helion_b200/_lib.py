@@ -142,19 +142,6 @@ def check(status: int, what: str) -> None:
         raise HelionB200Error(f"{what} failed with status {status}: {msg}")
 
 
-def entry(name: str):
-    """Entry point ``name`` as a function that raises on a non-zero status; looked up once, for calls whose host time
-    counts."""
-    fn = getattr(load(), name)
-
-    def run(*args) -> None:
-        status = fn(*args)
-        if status:
-            check(status, name)
-
-    return run
-
-
 def call(name: str, *args) -> None:
     """Invoke entry point ``name`` and raise on a non-zero status."""
     check(getattr(load(), name)(*args), name)

@@ -13,10 +13,12 @@ from . import _lib
 from .fused_linear import _cuda_getCurrentRawStream
 from .fused_linear import _cuda_getDevice
 from .fused_linear import _direct
+from .fused_linear import _empty
 from .ops import _require_cuda
 
 _SCORINGS = {"softmax": 0, "sigmoid": 1}
 _ARGS = struct.Struct("=11q3if")  # hb200_route_args
+_pack = _ARGS.pack
 _LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -65,15 +67,15 @@ def _route_cuda(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | 
                 group_top: int, renormalize: bool, scale: float) -> tuple[Tensor, Tensor]:
     global _entry
     _check(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top)
-    if not router_logits.is_cuda:
-        _require_cuda(router_logits)
     index = router_logits.get_device()
+    if index < 0:
+        _require_cuda(router_logits)
     if _cuda_getDevice() != index:
         with torch.cuda.device(index):
             return _route_cuda(router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
     tokens, experts = router_logits.shape
-    weights = router_logits.new_empty((tokens, top_k), dtype=torch.float32)
-    chosen = router_logits.new_empty((tokens, top_k), dtype=torch.int64)
+    weights = _empty((tokens, top_k), (top_k, 1), torch.float32)
+    chosen = _empty((tokens, top_k), (top_k, 1), torch.int64)
     if tokens == 0:
         return weights, chosen
     pitch, unit = router_logits.stride()
@@ -85,13 +87,14 @@ def _route_cuda(router_logits: Tensor, top_k: int, scoring: str, bias: Tensor | 
         bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
     if _entry is None:
-        _entry = _lib.entry("hb200_moe_route_experts")
-    _entry(
-        _ARGS.pack(router_logits.data_ptr(), bias_ptr, weights.data_ptr(), chosen.data_ptr(), tokens, experts, pitch, top_k,
-                   num_groups, top_groups, group_top, _LOGIT_DTYPES[router_logits.dtype], _SCORINGS[scoring], renormalize,
-                   scale),
+        _entry = _lib.load().hb200_moe_route_experts
+    status = _entry(
+        _pack(router_logits.data_ptr(), bias_ptr, weights.data_ptr(), chosen.data_ptr(), tokens, experts, pitch, top_k,
+              num_groups, top_groups, group_top, _LOGIT_DTYPES[router_logits.dtype], _SCORINGS[scoring], renormalize, scale),
         _cuda_getCurrentRawStream(index),
     )
+    if status:
+        _lib.check(status, "hb200_moe_route_experts")
     return weights, chosen
 
 

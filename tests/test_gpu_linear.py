@@ -324,3 +324,12 @@ def test_function_transforms():
     for got, plain in zip(torch.func.functionalize(lambda b: hb.route_experts(logits, 3, bias=b))(bias),
                           hb.route_experts(logits, 3, bias=bias)):
         assert torch.equal(got, plain)
+
+
+def test_outputs_under_inference_mode():
+    a, out = make(3, 40, 64)
+    with torch.inference_mode():
+        y = call(a, out)
+        weights, experts = hb.route_experts(torch.randn(3, 16, device=DEV), 2)
+    assert y.is_inference() and weights.is_inference() and experts.is_inference()
+    assert y.device == a["x"].device and torch.equal(y, call(a, out))
