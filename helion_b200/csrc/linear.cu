@@ -169,13 +169,20 @@ __device__ __forceinline__ void store8(OutT* p, int valid, bool vec, const float
 }
 
 // ------------------------------------------------------------------ tensor core
-__device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
+// Shared-memory descriptors are the low word of the operand's address (with the leading offset) under one constant
+// high word (stride 1024 bytes, descriptor version, 128-byte swizzle): the issue loop adds to low words only, so one
+// MMA costs it a handful of instructions, fewer than the 128 clocks the MMA runs.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | (1u << 16); }
+
+__device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
 
@@ -216,11 +223,19 @@ __device__ __forceinline__ void drain_mmas(uint32_t bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity) && clock64() - t0 < 20000000) {}
 }
 
+// The tensor core truncates every addition to its accumulator, so a sum drifts towards zero with the length of its
+// chain: 1e-9 of the result per element of K (3.8e-6 at 3584, 3.3e-5 at 28672).  That is invisible under a 16-bit
+// rounding, but up to 200 times the error of an fp32 product.  For fp32 outputs a chain is this many blocks of 64
+// elements (7e-7), and the partial sums are added outside the tensor core, to nearest, while the next chain runs in a
+// second accumulator.  4096^3: 125 us against 112 in one chain (a tile's epilogue hides behind two chains only); chains
+// of 8 blocks 130 us and 5e-7, of 24 118 us and 1.5e-6.
+constexpr int kChainBlocks = 12;
+
 // ------------------------------------------------------------------ streaming kernel
 constexpr int kStreamThreads = 192;
 constexpr int kTileRows = 128;                 // weight rows per tile
 constexpr int kWBytes = kTileRows * 128;       // one stage of weights: 128 rows x 64 elements
-constexpr int kMaxCols = 256;
+constexpr int kMaxCols = 128;                  // rows of x per tile: 256 took 13 us where 128 takes 8 (512 x 128 x 4096)
 constexpr int kMaxStages = 12;
 constexpr int kMaxSplit = 8;
 
@@ -229,12 +244,14 @@ __global__ void __launch_bounds__(kStreamThreads)
 linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Args g) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kOutRows = GATED ? 64 : 128;  // output columns per tile
+  constexpr bool kSums = std::is_same<OutT, float>::value;  // sums over chains of K, see kChainBlocks
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(base);
   uint64_t* empty_bar = full_bar + kMaxStages;
-  uint64_t* done_bar = empty_bar + kMaxStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  uint64_t* sum_bar = empty_bar + kMaxStages;  // an accumulator's chain is complete
+  uint64_t* free_bar = sum_bar + 2;            // ... and read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(free_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* ring = base + 1024;
   float* stash = reinterpret_cast<float*>(ring + g.stash_offset);  // [rank][column of mine][128] partial sums
@@ -253,16 +270,21 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
-    mbar_init(smem_u32(done_bar), 1);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&sum_bar[a]), 1);
+      mbar_init(smem_u32(&free_bar[a]), 4);
+    }
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_x);
   }
-  uint32_t tmem_cols = 32;
+  uint32_t tmem_cols = 32;  // of one accumulator
   while (tmem_cols < uint32_t(g.cols)) tmem_cols *= 2;
+  // two accumulators that take turns, then the sums of the chains before them; or one accumulator
+  const uint32_t tmem_all = kSums ? 4 * tmem_cols : tmem_cols;
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), tmem_cols);
+    tmem_alloc(smem_u32(tmem_slot), tmem_all);
     tmem_relinquish();
   }
   tcgen05_fence_before();
@@ -270,16 +292,17 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   wait_for_previous_kernel();
+  const int last_chain = kSums ? (kb1 - kb0 - 1) / kChainBlocks : 0;
   // A CTA's shared memory may be written by its peers once it runs (or, where the partial sums take the ring's
   // place, once its MMAs have read the ring): arrive here or below, wait in front of the first remote store.
   if (!overlay) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
   if (warp == 0) {
     const uint32_t bytes = uint32_t(kWBytes + g.cols * 128);
-    int it = 0;
+    int it = 0, s = 0;
+    uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb, ++it) {
-      const int s = it % g.stages;
-      if (!warp_wait(smem_u32(&empty_bar[s]), ((it / g.stages) & 1) ^ 1, abort_flag)) break;
+      if (!warp_wait(smem_u32(&empty_bar[s]), phase ^ 1, abort_flag)) break;
       if (elect_one()) {
         const uint32_t bar = smem_u32(&full_bar[s]);
         uint8_t* st = ring + s * g.stage_bytes;
@@ -289,34 +312,76 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         tma_load_2d(smem_u32(st + kWBytes), &tmap_x, kb * 64, m0, bar);
       }
       __syncwarp();
+      if (++s == g.stages) s = 0, phase ^= 1;
     }
     if (*abort_flag) drain_loads(full_bar, g.stages, it);
   } else if (warp == 1) {
     const uint32_t idesc = make_idesc(kTileRows, g.cols, kBf16);
+    const uint32_t ring_low = desc_low(smem_u32(ring)), stage_low = uint32_t(g.stage_bytes) >> 4;
+    const int tail_steps = (g.k - (g.num_kb - 1) * 64 + 15) / 16;  // K tail: TMA zero-fills past K
     bool ok = true;
-    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-      const int s = it % g.stages;
-      if (!warp_wait(smem_u32(&full_bar[s]), (it / g.stages) & 1, abort_flag)) { ok = false; break; }
+    int link = 0, chains = 0;  // blocks of the current chain so far, chains before it
+    int s = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      uint32_t tmem_d = tmem_base;
+      if constexpr (kSums) {
+        tmem_d += (chains & 1) * tmem_cols;
+        if (link == 0 && !warp_wait(smem_u32(&free_bar[chains & 1]), ((chains >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+      }
+      if (!warp_wait(smem_u32(&full_bar[s]), phase, abort_flag)) { ok = false; break; }
       tcgen05_fence_after();
-      uint8_t* st = ring + s * g.stage_bytes;
-      const uint32_t w_addr = smem_u32(st), x_addr = smem_u32(st + kWBytes);
-      const int k_left = g.k - kb * 64;
-      const int steps = k_left >= 64 ? 4 : (k_left + 15) / 16;  // K tail: TMA zero-fills past K
+      const uint32_t w_low = ring_low + uint32_t(s) * stage_low, x_low = w_low + (kWBytes >> 4);
+      const uint32_t more = link != 0 ? 1u : 0u;
       if (elect_one()) {
-        for (int a = 0; a < steps; ++a) {
-          const uint64_t wdesc = make_smem_desc(w_addr + a * 32, 16, 1024, kSwizzle128B);
-          const uint64_t xdesc = make_smem_desc(x_addr + a * 32, 16, 1024, kSwizzle128B);
-          mma_f16(tmem_base, wdesc, xdesc, idesc, (kb != kb0 || a != 0) ? 1u : 0u);
+        if (kb != g.num_kb - 1 || tail_steps == 4) {
+          mma_f16(tmem_d, w_low, x_low, idesc, more);
+#pragma unroll
+          for (int a = 1; a < 4; ++a) mma_f16(tmem_d, w_low + a * 2, x_low + a * 2, idesc, 1u);
+        } else {
+          for (int a = 0; a < tail_steps; ++a) mma_f16(tmem_d, w_low + a * 2, x_low + a * 2, idesc, more | uint32_t(a));
         }
         tcgen05_commit(smem_u32(&empty_bar[s]));
+        if (kb == kb1 - 1 || (kSums && link == kChainBlocks - 1)) tcgen05_commit(smem_u32(&sum_bar[chains & 1]));
       }
       __syncwarp();
+      ++link;
+      if (kSums && link == kChainBlocks) link = 0, ++chains;
+      if (++s == g.stages) s = 0, phase ^= 1;
     }
-    if (elect_one()) tcgen05_commit(smem_u32(done_bar));
-    __syncwarp();
-    if (!ok) drain_mmas(smem_u32(done_bar), 0);
+    if (!ok) {
+      if (elect_one()) tcgen05_commit(smem_u32(&sum_bar[chains & 1]));
+      __syncwarp();
+      drain_mmas(smem_u32(&sum_bar[chains & 1]), (chains >> 1) & 1);
+    }
   } else {
-    warp_wait(smem_u32(done_bar), 0, abort_flag);
+    bool ok = true;
+    if constexpr (kSums) {  // all chains but the last: into the sums
+      const uint32_t taddr = tmem_base + (uint32_t((warp & 3) * 32) << 16);
+      for (int chain = 0; chain < last_chain && ok; ++chain) {
+        ok = warp_wait(smem_u32(&sum_bar[chain & 1]), (chain >> 1) & 1, abort_flag);
+        tcgen05_fence_after();
+#pragma unroll 1
+        for (int c0 = 0; c0 < live_cols; c0 += 16) {
+          uint32_t r[16], t[16];
+          tmem_ld_32x32b_x16(taddr + (chain & 1) * tmem_cols + c0, r);
+          if (chain > 0) {
+            tmem_ld_32x32b_x16(taddr + 2 * tmem_cols + c0, t);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(t[j]));
+          } else {
+            tmem_ld_wait();
+          }
+          tmem_st_32x32b_x16(taddr + 2 * tmem_cols + c0, r);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&free_bar[chain & 1]));
+      }
+    }
+    if (ok) warp_wait(smem_u32(&sum_bar[last_chain & 1]), (last_chain >> 1) & 1, abort_flag);
     tcgen05_fence_after();
   }
   __syncwarp();
@@ -332,8 +397,16 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 #pragma unroll 1
     for (int c0 = 0; c0 < live_cols; c0 += 8) {
       uint32_t r[8];
-      tmem_ld_32x32b_x8(taddr + c0, r);
-      tmem_ld_wait();
+      tmem_ld_32x32b_x8(taddr + (last_chain & 1) * tmem_cols + c0, r);
+      if (kSums && last_chain > 0) {
+        uint32_t t[8];
+        tmem_ld_32x32b_x8(taddr + 2 * tmem_cols + c0, t);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(t[j]));
+      } else {
+        tmem_ld_wait();
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (c0 + j < live_cols) st_cluster_f32(map_to_cta(mine + uint32_t(index) * 512u, uint32_t(owner)), __uint_as_float(r[j]));
@@ -390,7 +463,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_dealloc(tmem_base, tmem_cols);
+    tmem_dealloc(tmem_base, tmem_all);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicMin(&g_device_status_linear, HB200_ERR_DEVICE_TIMEOUT);
 }
@@ -422,12 +495,6 @@ constexpr int kAcc = 2;
 constexpr int kPairBand = 8;                   // row tiles per band: 8192^3 reads 1.06 GB of DRAM (4: 1.51 GB, 16: 1.23 GB)
 constexpr size_t kPairSmem = size_t(kPairRingBytes) + kEpilogueWarps * 2 * kBoxBytes + (2 * kPairMaxStages + 2 * kAcc) * 8 + 16 + 1024;
 static_assert(kPairSmem <= 232448, "shared memory budget exceeded");
-
-// Shared-memory descriptors are the low word of the operand's address (with the leading offset) under one constant
-// high word (stride 1024 bytes, descriptor version, 128-byte swizzle): the issue loop adds to low words only, so one
-// MMA costs it a handful of instructions, fewer than the 128 clocks the MMA runs.
-constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | (1u << 16); }
 
 __device__ __forceinline__ void mma_pair_f16(uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc,
                                              uint32_t accumulate) {
@@ -564,6 +631,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const int num_tiles = g.m_tiles * g.n_tiles;
   const int kb0 = SPLIT ? range_start(part, g.num_kb, 1 << split_log) : 0;
   const int kb1 = SPLIT ? range_start(part + 1, g.num_kb, 1 << split_log) : g.num_kb;
+  constexpr bool kSums = std::is_same<OutT, float>::value;  // sums over chains of K, see kChainBlocks
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < num_stages; ++s) {
@@ -622,15 +690,16 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       const int tail_steps = (g.k - (g.num_kb - 1) * 64 + 15) / 16;  // K tail: TMA zero-fills past K
       bool ok = true;
       uint32_t s = 0, phase = 0, tc = 0;
-      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++tc) {
-        const uint32_t acc = tc % kAcc, tmem_d = tmem_base + acc * 256;
-        if (!warp_wait(smem_u32(&tmem_empty_bar[acc]), ((tc / kAcc) & 1) ^ 1, abort_flag)) { ok = false; break; }
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+        int link = 0;  // blocks of the current chain so far; tc counts chains
         for (int kb = kb0; kb < kb1; ++kb) {
+          const uint32_t acc = tc % kAcc, tmem_d = tmem_base + acc * 256;
+          if (link == 0 && !warp_wait(smem_u32(&tmem_empty_bar[acc]), ((tc / kAcc) & 1) ^ 1, abort_flag)) { ok = false; break; }
           if (!warp_wait(smem_u32(&full_bar[s]), phase, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
           const uint32_t x_low = ring_low + s * uint32_t(stage_bytes >> 4), w_low = x_low + (kHalfBytes >> 4);
-          const bool last = kb == kb1 - 1;
-          const uint32_t more = kb != kb0 ? 1u : 0u;
+          const bool last = kb == kb1 - 1 || (kSums && link == kChainBlocks - 1);
+          const uint32_t more = link != 0 ? 1u : 0u;
           if (elect_one()) {
             if (kb != g.num_kb - 1 || tail_steps == 4) {
               mma_pair_f16(tmem_d, x_low, w_low, idesc, more);
@@ -644,8 +713,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           }
           __syncwarp();
           if (++s == uint32_t(num_stages)) s = 0, phase ^= 1;
+          ++link;
+          if (last) link = 0, ++tc;
         }
-        if (!ok) break;  // (keeps tc, the accumulator of the tile that was given up)
       }
       if (!ok) {
         const uint32_t bar = smem_u32(&tmem_full_bar[tc % kAcc]);
@@ -665,10 +735,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     uint32_t tc = 0;
     constexpr int kSub = kBlocks * kBoxesPer32;           // boxes of outputs per warp and tile
     uint32_t boxes_used = 0;                              // the two boxes take turns
-    for (int tile = pair; tile < num_tiles; tile += num_pairs, ++tc) {
+    for (int tile = pair; tile < num_tiles; tile += num_pairs) {
       int m_blk, n_blk;
       decode_tile(g, tile, m_blk, n_blk);
-      const int acc = tc % kAcc;
       const int row0 = m_blk * kPairTile + int(rank) * 128 + quarter * 32;
       const int col0 = n_blk * out_cols + cgroup * (32 * kBlocks);
       // this warp has columns to finish: the tile is that wide, and (split) they are this pair's
@@ -697,18 +766,43 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           else if (col0 + i * kBoxCols < g.n) fetch_box<OutT>(g, box, row0, col0 + i * kBoxCols, lane);
         }
       }
-      const bool ready = epilogue_wait(warp == 2, smem_u32(&tmem_full_bar[acc]), (tc / kAcc) & 1, abort_flag);
+      bool ready = epilogue_wait(warp == 2, smem_u32(&tmem_full_bar[tc % kAcc]), (tc / kAcc) & 1, abort_flag);
       if (!SPLIT && !ready) break;  // (split: the cluster's barriers are still to be met)
       tcgen05_fence_after();
-      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * 256 + cgroup * (32 * kBlocks);
+      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + cgroup * (32 * kBlocks);
       uint32_t r[2][32];  // two blocks of 32 columns (gated: gate and up)
-      tmem_ld_32x32b_x32(taddr, r[0]);
-      tmem_ld_32x32b_x32(taddr + (GATED ? out_cols : 32), r[1]);
+      tmem_ld_32x32b_x32(taddr + (tc % kAcc) * 256, r[0]);
+      tmem_ld_32x32b_x32(taddr + (tc % kAcc) * 256 + (GATED ? out_cols : 32), r[1]);
       tmem_ld_wait();
       // everything is in registers: hand the accumulator back
-      tcgen05_fence_before();
-      __syncwarp();
-      if (!SPLIT && lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[acc]), leader_rank));
+      auto hand_back = [&] {
+        tcgen05_fence_before();
+        __syncwarp();
+        if ((!SPLIT || kSums) && lane == 0)
+          mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[tc % kAcc]), leader_rank));
+        ++tc;
+      };
+      hand_back();
+      if constexpr (kSums) {
+#pragma unroll 1
+        for (int kb = kb0 + kChainBlocks; kb < kb1 && ready; kb += kChainBlocks) {
+          ready = epilogue_wait(warp == 2, smem_u32(&tmem_full_bar[tc % kAcc]), (tc / kAcc) & 1, abort_flag);
+          tcgen05_fence_after();
+#pragma unroll
+          for (int c0 = 0; c0 < 64; c0 += 8) {
+            uint32_t t[8];
+            tmem_ld_32x32b_x8(taddr + (tc % kAcc) * 256 + (c0 < 32 ? c0 : c0 - 32 + (GATED ? out_cols : 32)), t);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t& sum = r[c0 / 32][c0 % 32 + j];
+              sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(t[j]));
+            }
+          }
+          hand_back();
+        }
+        if (!SPLIT && !ready) break;
+      }
       if constexpr (SPLIT) {
         // groups per pair; slot = [source][group of mine][quarter][block of 32 columns], 4 KB each: 32 lanes x 16 bytes x 8
         const int own_log = 2 - split_log, owner = cgroup >> own_log, split = 1 << split_log;
@@ -923,8 +1017,8 @@ struct StreamPlan {
 // 28672: 64 tiles over 4 CTAs each 72.8 us, over 2 88.7, over 8 (more CTAs than places) 76.9.
 StreamPlan plan_stream(int64_t m, int64_t n, int64_t k, bool gated, int dev, int sms) {
   StreamPlan p{};
-  p.cols = m >= kMaxCols ? kMaxCols : int((m + 15) / 16 * 16);
-  p.m_chunks = int((m + p.cols - 1) / p.cols);
+  p.m_chunks = int((m + kMaxCols - 1) / kMaxCols);
+  p.cols = int(((m + p.m_chunks - 1) / p.m_chunks + 15) / 16 * 16);
   p.num_kb = int((k + 63) / 64);
   const int out_rows = gated ? 64 : 128;
   p.tiles = ((n + out_rows - 1) / out_rows) * p.m_chunks;
@@ -959,7 +1053,7 @@ struct PairPlan {
 // grid, mostly the best).  A pair takes 0.27 us per 64 elements of K and 256 columns, 0.215 for 192 and 0.20 for 128
 // (bound by what an SM gets out of L2, not by the MMAs), a third more when every SM is busy (the clock drops), 7 us for
 // launch, first loads and last epilogue, and 2 to 3 us for an exchange of partial sums.  The stream kernel is bound by
-// the weight's bytes at 5.3 TB/s or by 68 bytes per clock into an SM, and every wave of its CTAs pays for its start and its epilogue.
+// the weight's bytes at 4.8 TB/s or by 55 bytes per clock into an SM, and every wave of its CTAs pays for its start and its epilogue.
 PairPlan plan_pair(int64_t m, int64_t weight_rows, int64_t k, int dev, int sms, double* us) {
   constexpr int kCols[3] = {256, 192, 128};
   constexpr double kPerBlock[3] = {0.27, 0.215, 0.20}, kExchange[3] = {0.0, 2.0, 3.0};
@@ -988,9 +1082,9 @@ PairPlan plan_pair(int64_t m, int64_t weight_rows, int64_t k, int dev, int sms, 
 
 double stream_us(const StreamPlan& p, double weight_bytes, int sms) {
   const double waves = double((p.tiles * p.split + sms - 1) / sms);
-  const double feed = waves * p.num_kb / p.split * (kWBytes + p.cols * 128) / (68.0 * 1900.0);
-  const double memory = weight_bytes / 5.3e6;
-  return 1.1 * (waves * (4.0 + 0.03 * p.cols) + (memory > feed ? memory : feed));
+  const double feed = waves * p.num_kb / p.split * (kWBytes + p.cols * 128) / (55.0 * 1900.0);
+  const double memory = weight_bytes / 4.8e6;
+  return waves * (2.5 + 0.03 * p.cols) + (memory > feed ? memory : feed);
 }
 
 // A cluster of `size` CTAs, launched as a programmatic dependent of whatever precedes it on the stream.

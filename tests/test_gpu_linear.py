@@ -333,3 +333,16 @@ def test_outputs_under_inference_mode():
         weights, experts = hb.route_experts(torch.randn(3, 16, device=DEV), 2)
     assert y.is_inference() and weights.is_inference() and experts.is_inference()
     assert y.device == a["x"].device and torch.equal(y, call(a, out))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 28672), (7, 19000, 4104), (70, 256, 8200), (130, 200, 4096), (200, 1024, 16384),
+                                   (256, 19200, 2048), (520, 2304, 4616), (1100, 4999, 1032)])
+@pytest.mark.parametrize("activation", ["none", "silu_and_mul"])
+def test_long_sums_in_fp32_outputs_do_not_drift(m, n, k, activation):
+    """Products of one sign: every truncated addition errs towards zero, so a sum over all of K in one chain would be
+    off by up to K / 16 steps of 2^-24, more than the bound for chains of 768 elements allows from K = 4096 on."""
+    a, _ = make(m, n, k, activation=activation)
+    a["x"], a["weight"] = a["x"].abs() + 0.125, a["weight"].abs()
+    y = call(a, torch.float32)
+    check(y, **a)
+    assert torch.equal(y, call(a, torch.float32)) and status_ok()
