@@ -5,15 +5,15 @@
 // Everything between the accumulator and the one final rounding happens in fp32.
 //
 // linear_stream_kernel streams the WEIGHT through the tensor core's M side: a tile is 128 weight rows (64 gate and 64
-// up rows when gated) by up to 256 rows of x, and the accumulator holds y transposed (lane = weight row, column =
+// up rows when gated) by up to 128 rows of x, and the accumulator holds y transposed (lane = weight row, column =
 // row of x).  A decode step is bound by the weight's bytes, and one SM streams about 1/148 of the HBM bandwidth, so
 // the K range of a tile is split over a thread-block cluster of up to 8 CTAs until there are two CTAs for every SM
 // (one, where a tile is wider than 64 rows of x).  The partial sums meet in distributed shared memory: column c of the
 // tile belongs to rank c % split, every rank stores its fp32 partial of a column into the owner's shared memory, and
 // after one cluster barrier the owner adds them in rank order (ascending K: the result does not depend on timing) and
 // runs the epilogue.  No workspace, no counters, no atomics: calls on any streams and replays of any graphs are
-// independent of each other.  Measured: one row, 8192 x 28672, 72.8 us = 6.45 TB/s; 16 rows, gated 57344 x 8192,
-// 149.5 us = 6.29 TB/s (the copy bandwidth of this GPU is 6.54).
+// independent of each other.  Measured: one row, 8192 x 28672, 72 us = 6.5 TB/s; 16 rows, gated 57344 x 8192, 145 us =
+// 6.5 TB/s (the copy bandwidth of this GPU is 6.54).
 //
 // linear_pair_kernel takes over where x has more rows than that form can hide behind the weight (see plan_pair).
 //
@@ -224,12 +224,14 @@ __device__ __forceinline__ void drain_mmas(uint32_t bar, uint32_t parity) {
 }
 
 // The tensor core truncates every addition to its accumulator, so a sum drifts towards zero with the length of its
-// chain: 1e-9 of the result per element of K (3.8e-6 at 3584, 3.3e-5 at 28672).  That is invisible under a 16-bit
-// rounding, but up to 200 times the error of an fp32 product.  For fp32 outputs a chain is this many blocks of 64
-// elements (7e-7), and the partial sums are added outside the tensor core, to nearest, while the next chain runs in a
-// second accumulator.  4096^3: 125 us against 112 in one chain (a tile's epilogue hides behind two chains only); chains
-// of 8 blocks 130 us and 5e-7, of 24 118 us and 1.5e-6.
-constexpr int kChainBlocks = 12;
+// chain: 1e-9 of the result per element of K (3.8e-6 at 3584, 3.3e-5 at 28672), twice that in a gated product.  That is
+// invisible under a 16-bit rounding, but up to 200 times the error of an fp32 product.  For fp32 outputs a chain is
+// this many blocks of 64 elements (3e-7 to 7e-7 of the result), and the partial sums are added outside the tensor core,
+// to nearest, while the next chain runs in a second accumulator.  Short chains cost the stream kernel nothing; in the
+// pair kernel a tile's epilogue hides behind two chains of the next tile only: 4096^3 takes 112 us in one chain, 118 in
+// chains of 24 blocks, 125 of 12, 130 of 8.
+constexpr int kStreamChain = 4;
+template <bool GATED> constexpr int kPairChain = GATED ? 5 : 10;
 
 // ------------------------------------------------------------------ streaming kernel
 constexpr int kStreamThreads = 192;
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(kStreamThreads)
 linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Args g) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kOutRows = GATED ? 64 : 128;  // output columns per tile
-  constexpr bool kSums = std::is_same<OutT, float>::value;  // sums over chains of K, see kChainBlocks
+  constexpr bool kSums = std::is_same<OutT, float>::value;  // sums over chains of K
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(base);
@@ -292,7 +294,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   wait_for_previous_kernel();
-  const int last_chain = kSums ? (kb1 - kb0 - 1) / kChainBlocks : 0;
+  const int last_chain = kSums ? (kb1 - kb0 - 1) / kStreamChain : 0;
   // A CTA's shared memory may be written by its peers once it runs (or, where the partial sums take the ring's
   // place, once its MMAs have read the ring): arrive here or below, wait in front of the first remote store.
   if (!overlay) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -342,11 +344,11 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
           for (int a = 0; a < tail_steps; ++a) mma_f16(tmem_d, w_low + a * 2, x_low + a * 2, idesc, more | uint32_t(a));
         }
         tcgen05_commit(smem_u32(&empty_bar[s]));
-        if (kb == kb1 - 1 || (kSums && link == kChainBlocks - 1)) tcgen05_commit(smem_u32(&sum_bar[chains & 1]));
+        if (kb == kb1 - 1 || (kSums && link == kStreamChain - 1)) tcgen05_commit(smem_u32(&sum_bar[chains & 1]));
       }
       __syncwarp();
       ++link;
-      if (kSums && link == kChainBlocks) link = 0, ++chains;
+      if (kSums && link == kStreamChain) link = 0, ++chains;
       if (++s == g.stages) s = 0, phase ^= 1;
     }
     if (!ok) {
@@ -631,7 +633,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const int num_tiles = g.m_tiles * g.n_tiles;
   const int kb0 = SPLIT ? range_start(part, g.num_kb, 1 << split_log) : 0;
   const int kb1 = SPLIT ? range_start(part + 1, g.num_kb, 1 << split_log) : g.num_kb;
-  constexpr bool kSums = std::is_same<OutT, float>::value;  // sums over chains of K, see kChainBlocks
+  constexpr bool kSums = std::is_same<OutT, float>::value;  // sums over chains of K
+  constexpr int kChain = kPairChain<GATED>;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < num_stages; ++s) {
@@ -698,7 +701,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           if (!warp_wait(smem_u32(&full_bar[s]), phase, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
           const uint32_t x_low = ring_low + s * uint32_t(stage_bytes >> 4), w_low = x_low + (kHalfBytes >> 4);
-          const bool last = kb == kb1 - 1 || (kSums && link == kChainBlocks - 1);
+          const bool last = kb == kb1 - 1 || (kSums && link == kChain - 1);
           const uint32_t more = link != 0 ? 1u : 0u;
           if (elect_one()) {
             if (kb != g.num_kb - 1 || tail_steps == 4) {
@@ -785,7 +788,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       hand_back();
       if constexpr (kSums) {
 #pragma unroll 1
-        for (int kb = kb0 + kChainBlocks; kb < kb1 && ready; kb += kChainBlocks) {
+        for (int kb = kb0 + kChain; kb < kb1 && ready; kb += kChain) {
           ready = epilogue_wait(warp == 2, smem_u32(&tmem_full_bar[tc % kAcc]), (tc / kAcc) & 1, abort_flag);
           tcgen05_fence_after();
 #pragma unroll

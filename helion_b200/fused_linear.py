@@ -11,7 +11,9 @@ import struct
 
 import torch
 from torch import Tensor
+from torch import is_grad_enabled as _is_grad_enabled
 from torch._C import _are_functorch_transforms_active as _in_transform
+from torch.compiler import is_compiling as _is_compiling
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import _lib
@@ -30,15 +32,19 @@ _ACTIVATIONS = {
 }
 _cuda_getDevice = getattr(torch._C, "_cuda_getDevice", None)  # (absent in a build without CUDA, where nothing gets there)
 _cuda_getCurrentRawStream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_PLAIN = (Tensor, torch.nn.Parameter)
 _ARGS = struct.Struct("=12q6i")  # hb200_linear_args (a bytes object passes through ctypes at a fifth of 18 values' cost)
 _pack = _ARGS.pack
 
 
 def _check(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
-           out_dtype: torch.dtype) -> tuple[int, int, torch.Size]:
-    """Validates a call; returns the numbers of output columns and of weight rows, and x's shape."""
-    if activation not in _ACTIVATIONS:
+           out_dtype: torch.dtype) -> tuple[int, int, int, bool, torch.Size]:
+    """Validates a call; returns the number of output columns, the weight's rows, the activation's code and gating, and
+    x's shape."""
+    kind = _ACTIVATIONS.get(activation)
+    if kind is None:
         raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}; got {activation!r}")
+    code, gated = kind
     dtype, device, x_shape, w_shape = x.dtype, x.device, x.shape, weight.shape
     if (dtype is not torch.bfloat16 and dtype is not torch.float16) or weight.dtype is not dtype:
         raise TypeError(f"linear takes bfloat16 or float16 operands of one type, got {dtype} and {weight.dtype}")
@@ -46,12 +52,13 @@ def _check(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | No
         raise TypeError(f"out_dtype must be {dtype} or torch.float32, got {out_dtype}")
     if len(x_shape) < 1 or len(w_shape) != 2:
         raise ValueError(f"linear expects x [..., K] and weight [rows, K]; got {tuple(x_shape)} and {tuple(w_shape)}")
-    n, k = rows, _ = w_shape
+    rows, k = w_shape
     if x_shape[-1] != k:
         raise ValueError(f"weight {tuple(w_shape)} does not match x {tuple(x_shape)}")
     if k == 0 or k % 8:
         raise ValueError(f"K must be a positive multiple of 8, got {k}")
-    if _ACTIVATIONS[activation][1]:
+    n = rows
+    if gated:
         if rows % 2:
             raise ValueError(f"{activation} needs a gate half and an up half of the weight's rows; got {rows} rows")
         n = rows // 2
@@ -71,7 +78,7 @@ def _check(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | No
             raise TypeError(f"residual must be {out_dtype} (the output's type), got {residual.dtype}")
         if residual.device != device:
             raise ValueError(f"all tensors must be on one device, got {device} and {residual.device}")
-    return n, rows, x_shape
+    return n, rows, code, gated, x_shape
 
 
 def _tma_rows(t: Tensor, rows: int, k: int) -> tuple[Tensor, int, int]:
@@ -102,7 +109,7 @@ def _empty(size: tuple[int, ...], stride: tuple[int, ...], dtype: torch.dtype) -
 def _linear_cuda(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
                  out_dtype: torch.dtype) -> Tensor:
     global _entry
-    n, rows, x_shape = _check(x, weight, bias, residual, activation, out_dtype)
+    n, rows, code, gated, x_shape = _check(x, weight, bias, residual, activation, out_dtype)
     index = x.get_device()
     if index < 0:
         _require_cuda(x)
@@ -134,7 +141,6 @@ def _linear_cuda(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tenso
     if bias is not None:
         bias = bias.contiguous()
         bias_ptr, bias_f32 = bias.data_ptr(), bias.dtype is torch.float32
-    code, gated = _ACTIVATIONS[activation]
     if _entry is None:
         _entry = _lib.load().hb200_linear
     status = _entry(
@@ -163,11 +169,11 @@ def _direct(*tensors: Tensor | None) -> bool:
     """Whether a call can go straight to its kernel: nothing traces or transforms (the tensors of a ``torch.func``
     transform look plain but have no address), and no subclass or gradient is involved.  The dispatch of a registered
     operator written in Python costs more host time than a small call's kernel runs."""
-    if torch.compiler.is_compiling() or _get_current_dispatch_mode() is not None or _in_transform():
+    if _is_compiling() or _get_current_dispatch_mode() is not None or _in_transform():
         return False
-    grad = torch.is_grad_enabled()
+    grad = _is_grad_enabled()
     for t in tensors:
-        if t is not None and ((type(t) is not Tensor and type(t) is not torch.nn.Parameter) or (grad and t.requires_grad)):
+        if t is not None and (type(t) not in _PLAIN or (grad and t.requires_grad)):
             return False
     return True
 

@@ -30,13 +30,13 @@ def linear(x, weight, bias, activation, residual, out_dtype):
 
     The tensor core adds 16 products to the accumulator at a time and may truncate: K / 16 additions (and up to 32
     within the first and last and over the partial sums of a split K range), each off by at most 2^-23 of a running
-    sum that never exceeds sum |x w|.  For fp32 outputs a chain of such additions covers 768 elements of K; the chains'
-    sums are added to nearest, each addition off by 2^-24.  The epilogue's exponential is off by a few units, scaled by
-    its argument."""
+    sum that never exceeds sum |x w|.  For fp32 outputs a chain of such additions covers at most 640 elements of K; the
+    chains' sums (of 256 elements at least) are added to nearest, each addition off by 2^-24.  The epilogue's
+    exponential is off by a few units, scaled by its argument."""
     k = weight.shape[1]
     xd, wd = x.double().reshape(-1, k), weight.double()
     v = xd @ wd.t()
-    additions = k / 16 if out_dtype is not torch.float32 else min(k, 768) / 16 + k / 1536
+    additions = k / 16 if out_dtype is not torch.float32 else min(k, 640) / 16 + k / 512
     err = (additions + 32) * 2.0**-23 * (xd.abs() @ wd.abs().t())
     if bias is not None:
         v = v + bias.double()

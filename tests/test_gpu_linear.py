@@ -340,7 +340,7 @@ def test_outputs_under_inference_mode():
 @pytest.mark.parametrize("activation", ["none", "silu_and_mul"])
 def test_long_sums_in_fp32_outputs_do_not_drift(m, n, k, activation):
     """Products of one sign: every truncated addition errs towards zero, so a sum over all of K in one chain would be
-    off by up to K / 16 steps of 2^-24, more than the bound for chains of 768 elements allows from K = 4096 on."""
+    off by up to K / 16 steps of 2^-24, more than the bound for chains of at most 640 elements allows from K = 4096 on."""
     a, _ = make(m, n, k, activation=activation)
     a["x"], a["weight"] = a["x"].abs() + 0.125, a["weight"].abs()
     y = call(a, torch.float32)
