@@ -138,17 +138,14 @@ __device__ __forceinline__ float load_bias(const Args& g, int64_t i) {
 
 // Eight consecutive values of a row: one or two 16-byte accesses where alignment allows.
 template <typename OutT>
-__device__ __forceinline__ void load8(const OutT* p, int valid, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void load8(const OutT* p, int valid, bool vec, OutT (&v)[8]) {
   if (vec && valid >= 8) {
-    OutT t[8];
     constexpr int kPieces = int(sizeof(OutT)) / 2;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = widen(t[j]);
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < valid ? widen(p[j]) : 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = j < valid ? p[j] : cast_out<OutT>(0.f);
   }
 }
 
@@ -264,8 +261,30 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   const int tile = int(blockIdx.x) / split;
   const int m0 = (tile % g.m_chunks) * g.cols, n0 = (tile / g.m_chunks) * kOutRows;
   const int kb0 = range_start(rank, g.num_kb, split), kb1 = range_start(rank + 1, g.num_kb, split);
-  const int per = (g.cols + split - 1) / split;  // columns this rank owns, at most
-  const int live_cols = min(g.cols, g.m - m0);   // columns past the last row of x are never stored
+  const int live_cols = min(g.cols, g.m - m0);     // columns past the last row of x are never stored
+  const int per = (live_cols + split - 1) / split;  // a rank finishes columns rank, rank + split, ...: at most this many
+  const int count = (live_cols - rank + split - 1) / split;
+
+  // Epilogue items: eight neighbouring outputs of one column, the same eight for all of a thread's columns.  Their
+  // biases and the first residuals are requested before the sums are complete.
+  constexpr int kItemsPerCol = kOutRows / 8, kStep = kStreamThreads / kItemsPerCol;
+  const int piece = (threadIdx.x % kItemsPerCol) * 8, first = threadIdx.x / kItemsPerCol;
+  const int col = n0 + piece, valid = g.n - col;
+  float bias[8], bias_up[8];
+  __align__(16) OutT res[8];
+  auto fetch = [&](int i, OutT (&v)[8]) {
+    if (g.residual != nullptr && i < count && valid > 0)
+      load8(static_cast<const OutT*>(g.residual) + int64_t(m0 + i * split + rank) * g.ldr + col, valid, g.res_vec != 0, v);
+  };
+  auto prefetch = [&] {
+    fetch(first, res);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool some = g.bias != nullptr && j < valid;
+      bias[j] = some ? load_bias<T>(g, col + j) : 0.f;
+      bias_up[j] = GATED && some ? load_bias<T>(g, int64_t(g.n) + col + j) : 0.f;
+    }
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.stages; ++s) {
@@ -317,6 +336,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       if (++s == g.stages) s = 0, phase ^= 1;
     }
     if (*abort_flag) drain_loads(full_bar, g.stages, it);
+    prefetch();
   } else if (warp == 1) {
     const uint32_t idesc = make_idesc(kTileRows, g.cols, kBf16);
     const uint32_t ring_low = desc_low(smem_u32(ring)), stage_low = uint32_t(g.stage_bytes) >> 4;
@@ -356,7 +376,9 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       __syncwarp();
       drain_mmas(smem_u32(&sum_bar[chains & 1]), (chains >> 1) & 1);
     }
+    prefetch();
   } else {
+    prefetch();
     bool ok = true;
     if constexpr (kSums) {  // all chains but the last: into the sums
       const uint32_t taddr = tmem_base + (uint32_t((warp & 3) * 32) << 16);
@@ -395,7 +417,7 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     const int r_in = quarter * 32 + lane;  // weight row inside the tile = accumulator lane
     const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16);
     const uint32_t mine = smem_u32(stash) + uint32_t((rank * per) * 128 + r_in) * 4u;
-    int owner = 0, index = 0;  // of column c: c % split and c / split
+    int owner = 0, index = 0;  // of column c: c % split and c / split (in turn: runs would send all ranks to one at a time)
 #pragma unroll 1
     for (int c0 = 0; c0 < live_cols; c0 += 8) {
       uint32_t r[8];
@@ -421,16 +443,14 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   // Orders the remote stores before the loads below; after it nobody touches another CTA's shared memory again.
   cluster_sync_all();
 
-  // my i-th column is the tile's column i * split + rank; an item is eight consecutive outputs of one column
-  constexpr int kItemsPerCol = kOutRows / 8;
-  for (int item = threadIdx.x; item < per * kItemsPerCol; item += kStreamThreads) {
-    const int i = item / kItemsPerCol, piece = (item % kItemsPerCol) * 8;
-    const int row = m0 + i * split + rank, col = n0 + piece;
-    const int valid = g.n - col;
-    if (i * split + rank >= live_cols || valid <= 0) continue;
-    float res[8], acc[8], up[8];
-    if (g.residual != nullptr)
-      load8(static_cast<const OutT*>(g.residual) + int64_t(row) * g.ldr + col, valid, g.res_vec != 0, res);
+  // (not unrolled: a launch runs this code once, and its instructions come in at the speed of a cold cache)
+#pragma unroll 1
+  for (int i = first; i < count && valid > 0; i += kStep) {
+    __align__(16) OutT r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = res[j];
+    fetch(i + kStep, res);
+    float acc[8], up[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = up[j] = 0.f;
     for (int q = 0; q < split; ++q) {
@@ -445,20 +465,17 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         }
       }
     }
+    if (g.bias != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (g.bias != nullptr && j < valid) {
-        acc[j] += load_bias<T>(g, col + j);
-        if constexpr (GATED) up[j] += load_bias<T>(g, int64_t(g.n) + col + j);
-      }
+      for (int j = 0; j < 8; ++j) acc[j] += bias[j], up[j] += bias_up[j];
     }
     activate_all(acc, g.activation);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (GATED) acc[j] *= up[j];
-      if (g.residual != nullptr) acc[j] += res[j];
+      if (g.residual != nullptr) acc[j] += widen(r[j]);
     }
-    store8(static_cast<OutT*>(g.out) + int64_t(row) * g.ldo + col, valid, g.out_vec != 0, acc);
+    store8(static_cast<OutT*>(g.out) + int64_t(m0 + i * split + rank) * g.ldo + col, valid, g.out_vec != 0, acc);
   }
 
   tcgen05_fence_before();
