@@ -12,8 +12,8 @@
 // tile belongs to rank c % split, every rank stores its fp32 partial of a column into the owner's shared memory, and
 // after one cluster barrier the owner adds them in rank order (ascending K: the result does not depend on timing) and
 // runs the epilogue.  No workspace, no counters, no atomics: calls on any streams and replays of any graphs are
-// independent of each other.  Measured: one row, 8192 x 28672, 72 us = 6.5 TB/s; 16 rows, gated 57344 x 8192, 145 us =
-// 6.5 TB/s (the copy bandwidth of this GPU is 6.54).
+// independent of each other.  Measured: one row, 8192 x 28672, 69-72 us = 6.5-6.8 TB/s; 16 rows, gated 57344 x 8192,
+// 140-145 us = 6.5-6.7 TB/s (a copy runs at 6.54).
 //
 // linear_pair_kernel takes over where x has more rows than that form can hide behind the weight (see plan_pair).
 //
