@@ -64,7 +64,9 @@ def test_sizes(m, n, k, activation):
 # sizes at which each form of the CTA-pair kernel runs on 148 SMs: tiles 256, 192 and 128 columns wide, K whole or split
 # over two or four pairs, tiles in one wave and in several
 FORMS = [(2048, 4096, 128), (640, 4096, 2040), (256, 9000, 512), (512, 4096, 4088), (768, 1536, 4096), (256, 4096, 4096),
-         (640, 1024, 4096), (512, 1024, 4088), (512, 512, 4096), (300, 520, 3584), (70, 8200, 1032)]
+         (640, 1024, 4096), (512, 1024, 4088), (512, 512, 4096), (300, 520, 3584), (70, 8200, 1032),
+         (266, 7136, 72), (283, 14280, 72), (132, 9488, 72), (281, 10408, 72), (6315, 536, 72), (4303, 264, 3192),
+         (5185, 208, 1928), (5127, 136, 1528), (4858, 128, 9952), (2061, 200, 4840), (2161, 136, 3704)]
 
 
 @pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
@@ -91,7 +93,7 @@ def test_pair_forms(m, n, k, activation, dtype, out):
 
 @pytest.mark.parametrize("activation", ACTIVATIONS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("m,n,k", [(3, 77, 128), (70, 264, 640), (700, 520, 264)])
+@pytest.mark.parametrize("m,n,k", [(3, 77, 128), (70, 264, 640), (700, 520, 264), (266, 7136, 72)])
 def test_activations_and_types(m, n, k, dtype, activation):
     for bias, residual, out in ((None, False, dtype), (dtype, True, dtype), (torch.float32, True, torch.float32)):
         a, out = make(m, n, k, dtype, activation, bias, residual, out)
@@ -102,7 +104,7 @@ def test_activations_and_types(m, n, k, dtype, activation):
 
 @pytest.mark.parametrize("activation", ["gelu_tanh", "silu_and_mul"])
 @pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
-@pytest.mark.parametrize("m,n,k", [(9, 333, 72), (90, 131, 200), (433, 387, 328), (1537, 641, 1032)])
+@pytest.mark.parametrize("m,n,k", [(9, 333, 72), (90, 131, 200), (433, 387, 328), (1537, 641, 1032), (283, 7139, 72)])
 def test_odd_widths_in_every_output_type(m, n, k, dtype, out, activation):
     a, out = make(m, n, k, dtype, activation, torch.float32, True, out)
     y = call(a, out)
@@ -113,9 +115,9 @@ def test_odd_widths_in_every_output_type(m, n, k, dtype, out, activation):
     assert torch.equal(call({**a, "residual": wide[:, 2 : 2 + n]}, out), y)
 
 
-@pytest.mark.parametrize("m", [1, 40, 600])
-def test_strides_and_shapes(m):
-    a, out = make(m, 136, 256, bias=torch.bfloat16, residual=True)
+@pytest.mark.parametrize("m,n", [(1, 136), (40, 136), (600, 136), (266, 7136)])
+def test_strides_and_shapes(m, n):
+    a, out = make(m, n, 256, bias=torch.bfloat16, residual=True)
     want = call(a, out)
     wide = torch.full((m, 256 + 72), float("nan"), dtype=torch.bfloat16, device=DEV)
     wide[:, 8:264] = a["x"]
@@ -124,12 +126,12 @@ def test_strides_and_shapes(m):
     assert torch.equal(call({**a, "x": wide[:, 3:259]}, out), want)  # rows off the 16-byte grid
     assert torch.equal(call({**a, "x": a["x"].t().contiguous().t()}, out), want)
     assert torch.equal(call({**a, "weight": a["weight"].t().contiguous().t()}, out), want)
-    tall = torch.full((137, 264), float("nan"), dtype=torch.bfloat16, device=DEV)
+    tall = torch.full((n + 1, 264), float("nan"), dtype=torch.bfloat16, device=DEV)
     tall[1:, :256] = a["weight"]
     assert torch.equal(call({**a, "weight": tall[1:, :256]}, out), want)
-    res = torch.full((m, 150), float("nan"), dtype=torch.bfloat16, device=DEV)
-    res[:, 5:141] = a["residual"]
-    assert torch.equal(call({**a, "residual": res[:, 5:141]}, out), want)
+    res = torch.full((m, n + 14), float("nan"), dtype=torch.bfloat16, device=DEV)
+    res[:, 5 : n + 5] = a["residual"]
+    assert torch.equal(call({**a, "residual": res[:, 5 : n + 5]}, out), want)
     assert torch.equal(call({**a, "residual": a["residual"].t().contiguous().t()}, out), want)
     assert torch.equal(call({**a, "bias": torch.stack([a["bias"], a["bias"]], 1)[:, 1]}, out), want)
     one = a["residual"][:1].expand(m, -1)  # one residual row for all
@@ -137,8 +139,8 @@ def test_strides_and_shapes(m):
     same = a["x"][:1].expand(m, -1)  # one row of x for all
     check(call({**a, "x": same}, out), **{**a, "x": same})
     if m % 2 == 0:
-        y = hb.linear(a["x"].view(2, m // 2, 256), a["weight"], a["bias"], residual=a["residual"].view(2, m // 2, 136))
-        assert torch.equal(y.view(m, 136), want)
+        y = hb.linear(a["x"].view(2, m // 2, 256), a["weight"], a["bias"], residual=a["residual"].view(2, m // 2, n))
+        assert torch.equal(y.view(m, n), want)
     assert torch.equal(hb.linear(a["x"][0], a["weight"]), hb.linear(a["x"][:1], a["weight"])[0])
     assert status_ok()
 
@@ -150,16 +152,16 @@ def test_empty():
     assert hb.linear(torch.zeros(3, 64, dtype=torch.float16, device=DEV), w[:0]).shape == (3, 0)
 
 
-@pytest.mark.parametrize("m", [2, 500])
-def test_infinities_and_nan_stay_in_their_rows_and_columns(m):
-    a, out = make(m, 300, 264)
+@pytest.mark.parametrize("m,n", [(2, 300), (500, 300), (300, 7136)])
+def test_infinities_and_nan_stay_in_their_rows_and_columns(m, n):
+    a, out = make(m, n, 264)
     clean = call(a, out)
     a["x"][1, 5] = float("nan")
     a["weight"][7, 100] = float("inf")
     y = call(a, out)
     assert torch.isnan(y[1]).all()
     rows = torch.arange(m, device=DEV) != 1
-    cols = torch.arange(300, device=DEV) != 7
+    cols = torch.arange(n, device=DEV) != 7
     assert torch.equal(y[rows][:, cols], clean[rows][:, cols])
     assert not torch.isfinite(y[:, 7]).any()
     relu = call({**a, "activation": "relu"}, out)
@@ -168,7 +170,8 @@ def test_infinities_and_nan_stay_in_their_rows_and_columns(m):
 
 def test_rows_past_the_edges_are_not_written_and_calls_repeat():
     lib = _lib.load()
-    for m, n, k in ((3, 100, 64), (270, 300, 72), (500, 300, 72), (500, 257, 72), (500, 304, 72)):
+    for m, n, k in ((3, 100, 64), (270, 300, 72), (500, 300, 72), (500, 257, 72), (500, 304, 72), (270, 7500, 72),
+                    (270, 7497, 72), (270, 7504, 72), (2061, 203, 4840)):
         a, _ = make(m, n, k)
         ldo = n + 20 if n % 8 else n + 24  # (row pitches on and off the 16-byte grid)
         out = torch.full((m + 2, ldo), 7.0, dtype=torch.bfloat16, device=DEV)
@@ -188,6 +191,7 @@ def test_rows_past_the_edges_are_not_written_and_calls_repeat():
 
 def test_streams_and_graphs_are_independent():
     cases = [make(m, 520, 1024, activation="gelu", residual=True, seed=s) for s, m in enumerate((1, 24, 90, 700))]
+    cases += [make(2061, 200, 4840, residual=True), make(266, 7136, 264, activation="silu_and_mul")]
     want = [call(a, out) for a, out in cases]
     streams = [torch.cuda.Stream() for _ in cases]
     torch.cuda.synchronize()
@@ -228,6 +232,8 @@ def test_operands_written_by_the_kernel_in_front():
     b8 = [(torch.randn(1024, 512, generator=g, device=DEV) * 0.05).to(torch.float8_e4m3fn) for _ in range(2)]
     one = torch.ones(1, device=DEV)
     buf, weight8 = torch.empty_like(x), torch.empty_like(b8[0])
+    tall = normal(7136, 512, std=512**-0.5)
+    tall_now = torch.empty_like(tall)
     c = torch.empty(16, 1024, dtype=torch.bfloat16, device=DEV)
 
     def chain(sync):
@@ -250,7 +256,11 @@ def test_operands_written_by_the_kernel_in_front():
             wait()
             hb.scaled_mm(c, a8, weight8.t(), one, one)  # its weight was written before the linear call in front of it
             wait()
-            out += [y, z, u, v, c.clone()]
+            torch.mul(tall, float(step), out=tall_now)
+            wait()
+            p = hb.linear(y[:300], tall_now)
+            wait()
+            out += [y, z, u, v, c.clone(), p]
             wait()
             w, r = (y * 0.05).to(torch.bfloat16), y
         return out
