@@ -283,7 +283,7 @@ import torch
 import helion_b200 as hb
 torch.manual_seed(0)
 cases = []
-for m, n, k in ((1, 256, 512), (100, 8192, 1024), (512, 1024, 4096), (2048, 2048, 512)):
+for m, n, k in ((1, 256, 512), (100, 8192, 1024), (512, 1024, 4096), (2048, 2048, 512), (2064, 200, 4840)):
     x = torch.randn(m, k, device="cuda").to(torch.bfloat16)
     cases.append((x, (torch.randn(n, k, device="cuda") / k**0.5).to(torch.bfloat16)))
 logits = torch.randn(20000, 64, device="cuda")
