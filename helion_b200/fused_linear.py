@@ -95,7 +95,7 @@ def _tma_rows(t: Tensor, rows: int, k: int) -> tuple[Tensor, int, int]:
 
 
 _entry = None
-_allocate = getattr(getattr(torch._C._dynamo, "guards", None), "_empty_strided_cuda", None)
+_allocate = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 
 def _empty(size: tuple[int, ...], stride: tuple[int, ...], dtype: torch.dtype) -> Tensor:
