@@ -508,24 +508,36 @@ __device__ __forceinline__ void route_token(const Args& a, int64_t token, const 
     if (lane == a.top_k - 1) next = left;
     // in units of the keys' values: the choices' error, and two for the values' own rounding
     const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 2.f);
-    bool close = has_pick && (next >> kIndexBits) != 0 && float((pick >> kIndexBits) - (next >> kIndexBits)) <= margin;
-    if (__any_sync(kAll, close)) {
-      if (close) {  // equal inputs are a tie whatever the precision
+    const bool near = has_pick && (next >> kIndexBits) != 0 && float((pick >> kIndexBits) - (next >> kIndexBits)) <= margin;
+    const unsigned near_picks = __ballot_sync(kAll, near);
+    if (near_picks != 0) {
+      auto bias_of = [&](int e) { return biased ? a.bias[e] : 0.f; };
+      bool unlike = near;
+      if (near) {  // equal inputs are a tie whatever the precision, and in their order already
         const int e = int(kIndexMask - (next & kIndexMask));
-        const float bias = biased ? a.bias[p.expert] : 0.f, next_bias = biased ? a.bias[e] : 0.f;
-        close = !(p.logit == float(row[e]) && bias == next_bias);
+        unlike = !(p.logit == float(row[e]) && bias_of(p.expert) == bias_of(e));
       }
-      const unsigned pairs = __ballot_sync(kAll, close);
-      if (pairs != 0) {
-        int count = a.top_k;
-        if ((pairs >> (a.top_k - 1)) & 1u) {  // the last pick and the one left behind: that one takes part too
-          const uint32_t beyond = __reduce_max_sync(kAll, m1);
-          count = a.top_k + 1;
-          slow = count > 32 || ((beyond >> kIndexBits) != 0 && float((left >> kIndexBits) - (beyond >> kIndexBits)) <= margin);
-          if (lane == a.top_k) p.expert = int(kIndexMask - (left & kIndexMask)), p.logit = float(row[p.expert]);
+      const bool some = __any_sync(kAll, unlike);
+      int count = a.top_k;
+      if ((near_picks >> (a.top_k - 1)) & 1u) {
+        // The last pick and the expert left behind are near each other, equal or not: what follows that one within the
+        // margin may come before both.  Only where all of these have the same inputs is it known which of them is picked.
+        const int e_left = int(kIndexMask - (left & kIndexMask));
+        const float l_left = float(row[e_left]), b_left = bias_of(e_left);
+        bool more = false, other = false;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+          if (alive && key[j] < left && (key[j] >> kIndexBits) != 0 && float((left >> kIndexBits) - (key[j] >> kIndexBits)) <= margin) {
+            const int e = lane * VPL + j;
+            more = true;
+            other |= !(float(row[e]) == l_left && bias_of(e) == b_left);
+          }
         }
-        if (!slow) p = refine_picks<T>(a, row, top, p, count);
+        count = a.top_k + 1;  // the one left behind takes part
+        slow = __any_sync(kAll, some ? more || count > 32 : other);
+        if (lane == a.top_k) p.expert = e_left, p.logit = l_left;
       }
+      if (some && !slow) p = refine_picks<T>(a, row, top, p, count);
     }
   }
   if (slow) p = choose_exactly<T, VPL>(a, row, lane);

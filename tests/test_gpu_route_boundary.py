@@ -1,0 +1,93 @@
+"""The end of the expert router's picks: equal inputs there, masks that are large but finite, scores that saturate."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import helion_b200 as hb
+from route_exact import picks
+from route_reference import route
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def check(logits, top_k, **kw):
+    """Indices against the definition, row by row where there are few of them."""
+    _, e = hb.route_experts(logits, top_k, **kw)
+    want = route(logits, top_k, **kw)[1] if logits.shape[0] <= 64 else picks(logits, top_k, **kw).cpu()
+    wrong = (e.cpu() != want).any(1).nonzero().flatten().tolist()
+    assert not wrong, f"{len(wrong)} rows, the first {wrong[0]}: {e[wrong[0]].tolist()}, not {want[wrong[0]].tolist()}"
+
+
+def tied_rows(tokens, experts, dtype, top_k, mask, seed, step=0.25):
+    """Logits on a grid, so that the last pick often has its equal behind it; the tail is padding with a finite mask."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    logits = (torch.randn(tokens, experts, generator=g, device=DEV) * 1.5 / step).round() * step
+    logits = logits.to(dtype)
+    if mask is not None:
+        logits[:, experts - max(1, experts // 8):] = mask
+        rows = torch.arange(0, tokens, 2, device=DEV)  # the first experts are equals around the place where the picks end
+        if top_k < experts - max(1, experts // 8):
+            logits[rows, top_k] = logits[rows, top_k - 1]
+    return logits
+
+
+# (experts, top_k, settings)
+CONFIGS = [
+    (16, 2, {}),
+    (32, 4, dict(scoring="sigmoid")),
+    (64, 6, dict(renormalize=True)),
+    (128, 8, {}),
+    (128, 8, dict(scoring="sigmoid", bias=0.25)),
+    (256, 8, dict(scoring="sigmoid", bias=0.5, num_groups=8, top_groups=4, group_top=2)),
+    (160, 6, dict(num_groups=8, top_groups=3)),
+    (384, 10, dict(scoring="sigmoid", bias=0.0)),
+    (1000, 32, {}),
+]
+
+
+def settings(experts, kw):
+    kw = dict(kw)
+    if "bias" in kw:
+        kw["bias"] = torch.full((experts,), kw["bias"], device=DEV)
+    return kw
+
+
+def masks(dtype):
+    return (None, -1e4, -65504.0) if dtype is torch.float16 else (None, -1e4, -1e9, -1e20)
+
+
+def test_a_tie_at_the_end_hides_nothing():
+    rows = [3, 1, 1, 9, 2, 4, 5, 6, 7, 8, 0, -1, -2, -3, -4, -1e9]
+    check(torch.tensor([rows], device=DEV, dtype=torch.float32), 2)
+    # scores that a step of 2^-24 cannot tell apart: two of them equal, the largest behind them
+    check(torch.tensor([[17.0, 17.0, 18.0]], device=DEV), 1, scoring="sigmoid", bias=torch.zeros(3, device=DEV))
+    # the last pick and the one behind it are equal, and both belong before the pick that stands in front of them
+    check(torch.tensor([[16.75, 17.0, 17.0, 3.0]], device=DEV), 2, scoring="sigmoid", bias=torch.zeros(4, device=DEV))
+    logits = torch.zeros(3, 64, device=DEV)  # one value alone, and one expert above or below it by a little
+    logits[1, 63], logits[2, 0] = 2.0**-20, -(2.0**-20)
+    for kw in ({}, dict(scoring="sigmoid"), dict(scoring="sigmoid", bias=torch.full((64,), 0.5, device=DEV))):
+        check(logits, 5, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("experts,top_k,kw", CONFIGS)
+def test_ties_and_finite_masks(experts, top_k, kw, dtype):
+    for i, mask in enumerate(masks(dtype)):
+        check(tied_rows(48, experts, dtype, top_k, mask, 10 * i + experts), top_k, **settings(experts, kw))
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,top_k", [(24, 3), (64, 6), (256, 8)])
+def test_saturated_scores_under_a_constant_bias(experts, top_k, scoring):
+    """Sigmoids next to 1 and softmax tails next to 0: fp32 choices are all alike, the 64-bit ones are not."""
+    g = torch.Generator(device=DEV).manual_seed(experts)
+    grid = torch.randint(0, 24, (48, experts), generator=g, device=DEV) * 0.25
+    logits = 15.0 + grid if scoring == "sigmoid" else grid - 20.0
+    if scoring == "softmax":
+        logits[:, experts // 2] = 4.0
+    check(logits, top_k, scoring=scoring, bias=torch.full((experts,), 0.25, device=DEV))
