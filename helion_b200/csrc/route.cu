@@ -792,15 +792,41 @@ route_many_kernel(const __grid_constant__ Args a) {
     const float logit = has_pick ? logit_of(expert) : -INFINITY;
     // one more than in route_token: what was left behind may lie below lo
     const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 3.f);
-    bool close = has_pick && next != 0 && float(value - next_value) <= margin;
+    const bool near = has_pick && next != 0 && float(value - next_value) <= margin;
+    bool close = near;
     if (__any_sync(kAll, close)) {
-      if (close) {  // equal inputs are a tie whatever the precision
+      if (close) {  // equal inputs are a tie whatever the precision, and in their order already
         const int e = min(int(kIndexMask - (next & kIndexMask)), a.experts - 1);
         close = !(next_value != 0 && logit == logit_of(e) && (!biased || a.bias[expert] == a.bias[e]));
       }
     }
     unsure |= has_pick && value == 0;
-    const unsigned unsure_lanes = __ballot_sync(kAll, unsure), close_lanes = __ballot_sync(kAll, close);
+    const unsigned close_lanes = __ballot_sync(kAll, close), edge_lanes = __ballot_sync(kAll, near && l8 == a.top_k - 1);
+    if (edge_lanes != 0) {
+      // The last pick and the expert left behind are near each other, equal or not: what follows that one within the
+      // margin may come before both.  Only where all of these have the same inputs is it known which of them is picked.
+      const uint32_t beyond = eight_max(m1), left_value = left >> kIndexBits;
+      const bool deep = ((edge_lanes >> (lane & 24)) & 255u) != 0 &&
+                        !(left_value != 0 && float(left_value - (beyond >> kIndexBits)) > margin);
+      if (__any_sync(kAll, deep)) {
+        bool other = false;
+        if (deep && alive) {
+          const int e_left = min(int(kIndexMask - (left & kIndexMask)), a.experts - 1);
+          const float l_left = logit_of(e_left), b_left = biased ? a.bias[e_left] : 0.f;
+#pragma unroll
+          for (int j = 0; j < VPL; ++j) {
+            const int e = l8 * VPL + j;
+            if (key[j] < left && float(left_value - (key[j] >> kIndexBits)) <= margin && e < a.experts) {
+              const float l = logit_of(e);
+              other |= l > -INFINITY && !(l == l_left && (!biased || a.bias[e] == b_left));
+            }
+          }
+        }
+        const unsigned others = __ballot_sync(kAll, other);
+        unsure |= deep && (((close_lanes | others) >> (lane & 24)) & 255u) != 0;
+      }
+    }
+    const unsigned unsure_lanes = __ballot_sync(kAll, unsure);
     const bool done = (((unsure_lanes | close_lanes) >> (lane & 24)) & 255u) == 0;
 
     // weights, as in write_weights
@@ -825,21 +851,16 @@ route_many_kernel(const __grid_constant__ Args a) {
     }
     __syncwarp();
     if ((unsure_lanes | close_lanes) != 0) {
-      const uint32_t beyond = eight_max(m1);
-      // the last pick and the one left behind are close: that one takes part, if it is clear of what comes after it
-      const bool clear = (left >> kIndexBits) != 0 && float((left >> kIndexBits) - (beyond >> kIndexBits)) > margin;
-      unsure = !clear && ((close_lanes >> ((lane & 24) + a.top_k - 1)) & 1u);
-      const unsigned tied = __ballot_sync(kAll, unsure);
       for (int t = 0; t < 4; ++t) {
         const unsigned close_t = (close_lanes >> (8 * t)) & 255u;
         if (first + t >= a.tokens) break;
-        if ((((unsure_lanes | tied) >> (8 * t)) & 255u) != 0) {
+        if (((unsure_lanes >> (8 * t)) & 255u) != 0) {
           route_token_apart<T, GROUPED ? kAnyGroups : kNoGroups>(a, first + t, scratch[GROUPED ? warp : 0]);
         } else if (close_t != 0) {
           const int source = 8 * t + (lane & 7);
           Picks p{__shfl_sync(kAll, expert, source), __shfl_sync(kAll, logit, source)};
           const uint32_t left_t = __shfl_sync(kAll, left, 8 * t);
-          const bool joins = (close_t >> (a.top_k - 1)) & 1u;
+          const bool joins = ((edge_lanes >> (8 * t)) & 255u) != 0;  // the one left behind takes part
           if (joins && lane == a.top_k) {
             p.expert = int(kIndexMask - (left_t & kIndexMask));
             p.logit = float(*reinterpret_cast<const T*>(staged[warp][buf] + t * kRowBytes + p.expert / VPL * kLaneBytes +

@@ -19,9 +19,9 @@ def picks(logits, top_k, *, scoring="softmax", bias=None, num_groups=1, top_grou
     if num_groups > 1:
         best = by_group.view(tokens, num_groups, -1).sort(2, descending=True).values[..., :group_top]
         total = best.masked_fill(best == -math.inf, 0.0).sum(2).masked_fill(best[..., 0] == -math.inf, -math.inf)
-        order = total.sort(1, descending=True, stable=True).indices[:, :top_groups]
+        order = total.sort(dim=1, descending=True, stable=True).indices[:, :top_groups]
         kept = torch.zeros(tokens, num_groups, dtype=torch.bool, device=z.device).scatter_(1, order, True)
         closed = ~kept.repeat_interleave(experts // num_groups, 1)
-    by_choice = choice.sort(1, descending=True, stable=True).indices
-    last = closed.gather(1, by_choice).sort(1, stable=True).indices  # closed experts behind all open ones
+    by_choice = choice.sort(dim=1, descending=True, stable=True).indices
+    last = closed.gather(1, by_choice).sort(dim=1, stable=True).indices  # closed experts behind all open ones
     return by_choice.gather(1, last)[:, :top_k]

@@ -2,8 +2,6 @@
 
 from __future__ import annotations
 
-import math
-
 import pytest
 import torch
 
@@ -87,6 +85,40 @@ def test_saturated_scores_under_a_constant_bias(experts, top_k, scoring):
     """Sigmoids next to 1 and softmax tails next to 0: fp32 choices are all alike, the 64-bit ones are not."""
     g = torch.Generator(device=DEV).manual_seed(experts)
     grid = torch.randint(0, 24, (48, experts), generator=g, device=DEV) * 0.25
+    logits = 15.0 + grid if scoring == "sigmoid" else grid - 20.0
+    if scoring == "softmax":
+        logits[:, experts // 2] = 4.0
+    check(logits, top_k, scoring=scoring, bias=torch.full((experts,), 0.25, device=DEV))
+
+
+MANY = [
+    (32, 2, {}),
+    (64, 6, dict(renormalize=True)),
+    (64, 8, dict(scoring="sigmoid", bias=0.5, num_groups=8, top_groups=4, group_top=2)),
+    (128, 8, {}),
+    (128, 1, dict(scoring="sigmoid", bias=0.25)),
+    (192, 8, dict(scoring="sigmoid", bias=0.25, num_groups=8, top_groups=4)),
+    (256, 8, dict(scoring="sigmoid")),
+    (256, 6, dict(scoring="sigmoid", bias=0.0, num_groups=8, top_groups=4, group_top=2)),
+    (256, 5, dict(num_groups=8, top_groups=3)),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("experts,top_k,kw", MANY)
+def test_ties_and_finite_masks_in_large_batches(experts, top_k, kw, dtype):
+    for i, mask in enumerate(masks(dtype)):
+        logits = tied_rows(16403, experts, dtype, top_k, mask, 10 * i + experts)
+        logits[5000:6000] = 0.0  # rows of padding, all of one value
+        logits[6000:6500, ::2] = -1.0
+        check(logits, top_k, **settings(experts, kw))
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,top_k", [(64, 6), (256, 8)])
+def test_saturated_scores_in_large_batches(experts, top_k, scoring):
+    g = torch.Generator(device=DEV).manual_seed(experts)
+    grid = torch.randint(0, 24, (16403, experts), generator=g, device=DEV) * 0.25
     logits = 15.0 + grid if scoring == "sigmoid" else grid - 20.0
     if scoring == "softmax":
         logits[:, experts // 2] = 4.0
