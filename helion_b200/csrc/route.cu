@@ -527,10 +527,11 @@ __device__ __forceinline__ void route_token(const Args& a, int64_t token, const 
         bool more = false, other = false;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-          if (alive && key[j] < left && (key[j] >> kIndexBits) != 0 && float((left >> kIndexBits) - (key[j] >> kIndexBits)) <= margin) {
-            const int e = lane * VPL + j;
-            more = true;
-            other |= !(float(row[e]) == l_left && bias_of(e) == b_left);
+          // (value 0 lies below lo, by how little is not known: it counts as lo itself)
+          const int e = lane * VPL + j;
+          if (alive && e < a.experts && key[j] < left && float((left >> kIndexBits) - max(key[j] >> kIndexBits, 1u)) <= margin) {
+            const float l = float(row[e]);
+            if (l > -INFINITY) more = true, other |= !(l == l_left && bias_of(e) == b_left);
           }
         }
         count = a.top_k + 1;  // the one left behind takes part

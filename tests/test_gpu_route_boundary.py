@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -123,3 +125,23 @@ def test_saturated_scores_in_large_batches(experts, top_k, scoring):
     if scoring == "softmax":
         logits[:, experts // 2] = 4.0
     check(logits, top_k, scoring=scoring, bias=torch.full((experts,), 0.25, device=DEV))
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_three_choices_within_rounding_at_the_bottom_of_the_range(scoring):
+    """As many lanes with experts as picks and one more, and a third choice next to the smallest of the lanes' best: the
+    last pick, the one left behind and that one meet to within 2^-25."""
+    g = torch.Generator().manual_seed(5)
+    behind = 0
+    for trial in range(200):
+        live = [0, 1, 2, 4]  # two experts to a lane: 0 leads, 1 shares its lane
+        logits = torch.full((64,), -math.inf)
+        logits[live] = torch.randn(4, generator=g)
+        score = torch.softmax(logits.double(), 0) if scoring == "softmax" else torch.sigmoid(logits.double())
+        bias = torch.zeros(64)
+        bias[live] = (0.75 - score[live]).float()
+        bias[0] += 0.25
+        exact = score + bias.double()
+        behind += int(exact[1] > min(exact[2], exact[4]))
+        check(logits[None].to(DEV), 2, scoring=scoring, bias=bias.to(DEV))
+    assert behind > 50  # the third one belongs among the picks often enough
