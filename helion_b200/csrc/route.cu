@@ -472,8 +472,8 @@ __device__ __forceinline__ void route_token(const Args& a, int64_t token, const 
     for (int j = 0; j < VPL; ++j) lo = c[j] > -INFINITY ? fminf(lo, c[j]) : lo;
     lo = redux_min(alive ? lo : INFINITY);
   }
-  const float range = hi - lo;
-  slow |= !(range < 1e30f);
+  const float range = hi - lo, largest = fmaxf(fabsf(hi), fabsf(lo));
+  slow |= !(largest < 1e30f);  // infinite, or so large that a group's sum may have left fp32
   const float scale = float((1 << kValueBits) - 600) * reciprocal_fast(fmaxf(range, 1e-30f));
   // value 0: below lo, masked or dropped; 1 and up: in the range.  Added to 2^23 it is the sum's last 23 bits, and
   // what 2^23 itself would leave in the key goes with the index's constant.
@@ -507,7 +507,7 @@ __device__ __forceinline__ void route_token(const Args& a, int64_t token, const 
     uint32_t next = __shfl_down_sync(kAll, pick, 1);
     if (lane == a.top_k - 1) next = left;
     // in units of the keys' values: the choices' error, and two for the values' own rounding
-    const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 2.f);
+    const float margin = fmaf(scale, base + largest * (1.f / (1 << 22)), 2.f);
     const bool near = has_pick && (next >> kIndexBits) != 0 && float((pick >> kIndexBits) - (next >> kIndexBits)) <= margin;
     const unsigned near_picks = __ballot_sync(kAll, near);
     if (near_picks != 0) {
@@ -755,8 +755,8 @@ route_many_kernel(const __grid_constant__ Args a) {
     lo = eight_min(lo);
     hi = eight_max_nan(alive ? hi : -INFINITY);
     lo -= 0.125f * (hi - lo);  // room below, so that what is left behind is not mistaken for a neighbour of the last pick
-    const float range = hi - lo;
-    unsure |= !(range < 1e30f);
+    const float range = hi - lo, largest = fmaxf(fabsf(hi), fabsf(lo));
+    unsure |= !(largest < 1e30f);
     const float scale = float((1 << kValueBits) - 600) * reciprocal_fast(fmaxf(range, 1e-30f));
     uint32_t key[VPL], m1 = 0, m2 = 0, m3 = 0, m4 = 0;
     const uint32_t index = kIndexMask - uint32_t(l8 * VPL) - (0x4b000000u << kIndexBits);
@@ -792,7 +792,7 @@ route_many_kernel(const __grid_constant__ Args a) {
     };
     const float logit = has_pick ? logit_of(expert) : -INFINITY;
     // one more than in route_token: what was left behind may lie below lo
-    const float margin = fmaf(scale, base + fmaxf(fabsf(hi), fabsf(lo)) * (1.f / (1 << 22)), 3.f);
+    const float margin = fmaf(scale, base + largest * (1.f / (1 << 22)), 3.f);
     const bool near = has_pick && next != 0 && float(value - next_value) <= margin;
     bool close = near;
     if (__any_sync(kAll, close)) {

@@ -145,3 +145,21 @@ def test_three_choices_within_rounding_at_the_bottom_of_the_range(scoring):
         behind += int(exact[1] > min(exact[2], exact[4]))
         check(logits[None].to(DEV), 2, scoring=scoring, bias=bias.to(DEV))
     assert behind > 50  # the third one belongs among the picks often enough
+
+
+@pytest.mark.parametrize("tokens", [3, 16403])
+@pytest.mark.parametrize("experts,groups", [(64, 8), (24, 8), (60, 12), (256, 32)])
+def test_group_scores_beyond_fp32(experts, groups, tokens):
+    """Sums of two choices that fp32 cannot hold, upwards and downwards: the larger sum is still the larger."""
+    g = torch.Generator(device=DEV).manual_seed(experts)
+    logits = torch.randn(tokens, experts, generator=g, device=DEV)
+    logits[1] = 0.5
+    size = experts // groups
+    for sign in (1, -1):
+        bias = torch.zeros(groups, size, device=DEV)
+        bias[1], bias[2] = sign * 3e38, sign * 2e38
+        bias[4] = 3.2e38  # (the largest where they are positive, alone in its group where they are negative)
+        if sign < 0:
+            bias[[0, *range(3, groups)]] = -3.2e38
+        for top_k in (2, size):
+            check(logits, top_k, scoring="sigmoid", bias=bias.flatten(), num_groups=groups, group_top=2)
