@@ -152,7 +152,7 @@ __device__ __forceinline__ void load8(const OutT* p, int valid, bool vec, OutT (
 template <typename OutT>
 __device__ __forceinline__ void store8(OutT* p, int valid, bool vec, const float (&v)[8]) {
   if (vec && valid >= 8) {
-    OutT t[8];
+    __align__(16) OutT t[8];
     constexpr int kPieces = int(sizeof(OutT)) / 2;
 #pragma unroll
     for (int j = 0; j < 8; ++j) t[j] = cast_out<OutT>(v[j]);

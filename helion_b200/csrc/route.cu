@@ -89,7 +89,7 @@ template <typename T, int VPL>
 __device__ __forceinline__ void load_row(const Args& a, const T* row, int lane, float (&l)[VPL]) {
   if (a.vec) {
     constexpr int kBytes = VPL * int(sizeof(T)), kWord = kBytes < 16 ? kBytes : 16;
-    T t[VPL];
+    __align__(16) T t[VPL];  // written in words of up to 16 bytes
     if (lane * VPL < a.experts) {
 #pragma unroll
       for (int i = 0; i < kBytes / kWord; ++i) {
