@@ -86,7 +86,8 @@ __device__ __forceinline__ float activate(float v, int activation) {
       p = fmaf(p, t, 0.10865677893161774f);
       p = fmaf(p, t, 0.12443558871746063f);
       p = fmaf(p, t, 0.12411047518253326f);
-      return fmaf(-a, exp2_fast(-0.5f * kLog2e * v * v) * (t * p), fmaxf(v, 0.f));
+      // (min(v, -a): -inf times a tail of 0 is NaN as in the formula, while the clamped a keeps +inf)
+      return fmaf(fminf(v, -a), exp2_fast(-0.5f * kLog2e * v * v) * (t * p), fmaxf(v, 0.f));
     }
     case kGeluTanh: {
       // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
