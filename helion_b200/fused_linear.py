@@ -13,6 +13,7 @@ import torch
 from torch import Tensor
 from torch import is_grad_enabled as _is_grad_enabled
 from torch._C import _are_functorch_transforms_active as _in_transform
+from torch._C import _is_tracing
 from torch.compiler import is_compiling as _is_compiling
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
@@ -166,10 +167,11 @@ def _(x, weight, bias, residual, activation, out_dtype):
 
 
 def _direct(*tensors: Tensor | None) -> bool:
-    """Whether a call can go straight to its kernel: nothing traces or transforms (the tensors of a ``torch.func``
-    transform look plain but have no address), and no subclass or gradient is involved.  The dispatch of a registered
-    operator written in Python costs more host time than a small call's kernel runs."""
-    if _is_compiling() or _get_current_dispatch_mode() is not None or _in_transform():
+    """Whether a call can go straight to its kernel: nothing traces (``torch.jit.trace`` would record the output's
+    allocation alone) or transforms (the tensors of a ``torch.func`` transform look plain but have no address), and no
+    subclass or gradient is involved.  The dispatch of a registered operator written in Python costs more host time than
+    a small call's kernel runs."""
+    if _is_compiling() or _is_tracing() or _get_current_dispatch_mode() is not None or _in_transform():
         return False
     grad = _is_grad_enabled()
     for t in tensors:

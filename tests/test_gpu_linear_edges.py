@@ -34,3 +34,21 @@ def test_activations_at_both_infinities(m, n, activation, out):
     step = torch.finfo(out).eps / 2 + 2.0**-19
     assert ((y.double() - want).abs() <= step * want.abs() + 2.0**-126).logical_or(~ok).all()
     assert torch.equal(y[:, torch.isinf(want)].double(), want[torch.isinf(want)].expand(m, -1))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+@pytest.mark.parametrize("shape", [(5, 64), (2, 3, 64)])
+def test_traced_calls_run_their_kernels(shape):
+    g = torch.Generator(device=DEV).manual_seed(1)
+    w = torch.randn(24, 64, generator=g, device=DEV).to(torch.bfloat16)
+
+    def block(x):
+        y = hb.linear(x, w, activation="silu", residual=x[..., :24])
+        return (y, *hb.route_experts(hb.linear(x, w, out_dtype=torch.float32).flatten(0, -2), 3, scoring="sigmoid"))
+
+    traced = torch.jit.trace(block, (torch.randn(shape, generator=g, device=DEV).to(torch.bfloat16),))
+    for _ in range(2):
+        x = torch.randn(shape, generator=g, device=DEV).to(torch.bfloat16)
+        junk = [torch.full_like(t, 7) for t in block(x)]  # (what an output that nothing writes would hold)
+        del junk
+        assert all(torch.equal(a, b) for a, b in zip(traced(x), block(x)))
