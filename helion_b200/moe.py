@@ -30,6 +30,7 @@ from .layouts import swizzled_scale_numel
 from .ops import _require_cuda
 from .ops import _stream
 from .routing import Routing
+from .routing import _check as _check_routing
 
 
 @dataclass
@@ -296,13 +297,22 @@ def _quantize_rows_amax(y: Tensor, row_amax: Tensor, k: int, sched: MoeSchedule,
     return codes, scales, gscale
 
 
+def _routing_of(scoring: str, bias: Tensor | None, num_groups: int, top_groups: int, group_top: int, renormalize: bool,
+                scale: float) -> Routing | None:
+    """The registered operator's routing.  No scoring and no setting: softmax and top-k alone (``route_top_k``)."""
+    if scoring:
+        return Routing(scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
+    if bias is not None or (num_groups, top_groups, group_top, renormalize, scale) != (1, 1, 1, False, 1.0):
+        raise ValueError(f"scoring must be 'softmax' or 'sigmoid' where routing settings are given; got {scoring!r}")
+    return None
+
+
 @torch.library.custom_op("helion_b200::nvfp4_moe", mutates_args=())
 def _nvfp4_moe_op(x: Tensor, router_logits: Tensor, top_k: int, gu_packed: Tensor, gu_scales: Tensor,
                   gu_global: Tensor, gu_interleaved: bool, d_packed: Tensor, d_scales: Tensor, d_global: Tensor,
                   scoring: str = "", route_bias: Tensor | None = None, num_groups: int = 1, top_groups: int = 1,
                   group_top: int = 1, renormalize: bool = False, route_scale: float = 1.0) -> Tensor:
-    # no scoring: softmax and top-k alone (route_top_k)
-    routing = Routing(scoring, route_bias, num_groups, top_groups, group_top, renormalize, route_scale) if scoring else None
+    routing = _routing_of(scoring, route_bias, num_groups, top_groups, group_top, renormalize, route_scale)
     return _nvfp4_moe_impl(x, router_logits, top_k, GroupedNvfp4Weight(gu_packed, gu_scales, gu_global, gu_interleaved),
                            GroupedNvfp4Weight(d_packed, d_scales, d_global), None, routing)
 
@@ -310,6 +320,7 @@ def _nvfp4_moe_op(x: Tensor, router_logits: Tensor, top_k: int, gu_packed: Tenso
 @_nvfp4_moe_op.register_fake
 def _(x, router_logits, top_k, gu_packed, gu_scales, gu_global, gu_interleaved, d_packed, d_scales, d_global, scoring="",
       route_bias=None, num_groups=1, top_groups=1, group_top=1, renormalize=False, route_scale=1.0):
+    _routing_of(scoring, route_bias, num_groups, top_groups, group_top, renormalize, route_scale)
     return x.new_empty(x.shape)
 
 
@@ -338,6 +349,9 @@ def nvfp4_moe(x: Tensor, router_logits: Tensor, top_k: int, w_gate_up: GroupedNv
     inter = w_gate_up.n // 2
     if w_gate_up.k != h or w_down.k != inter or w_down.n != h or w_down.experts != e:
         raise ValueError("expert weight shapes do not match the activations")
+    if routing is not None:
+        _check_routing(router_logits, top_k, routing.scoring, routing.bias, routing.num_groups, routing.top_groups,
+                       routing.group_top)
     if intermediates is not None:
         return _nvfp4_moe_impl(x, router_logits, top_k, w_gate_up, w_down, intermediates, routing)
     bundles = (w_gate_up.packed, w_gate_up.scales, w_gate_up.global_scale, w_gate_up.gate_up_interleaved, w_down.packed,
