@@ -655,6 +655,7 @@ class ExpertParallel:
 
         if x.shape != (self.tokens, self.hidden) or x.dtype is not torch.bfloat16 or not x.is_contiguous():
             raise ValueError(f"x must be a contiguous bfloat16 [{self.tokens}, {self.hidden}] tensor")
+        M._check_logits(router_logits, x, self.experts)
         weights, experts = (routing or M.route_top_k)(router_logits, self.top_k)
         codes_t, scales_t, g_t = ops.nvfp4_quantize(x)
         flat = experts.reshape(-1)

@@ -297,6 +297,16 @@ def _quantize_rows_amax(y: Tensor, row_amax: Tensor, k: int, sched: MoeSchedule,
     return codes, scales, gscale
 
 
+def _check_logits(router_logits: Tensor, x: Tensor, experts: int) -> None:
+    """A row of logits per token and no expert without weights: the schedule has no rows for anything else, and the
+    kernels behind it would follow entries that nothing wrote."""
+    tokens = x.shape[0]
+    if router_logits.dim() != 2 or router_logits.shape[0] != tokens or router_logits.shape[1] > experts:
+        raise ValueError(f"router_logits must be [{tokens}, {experts}], got {tuple(router_logits.shape)}")
+    if router_logits.device != x.device:
+        raise ValueError(f"all tensors must be on one device, got {x.device} and {router_logits.device}")
+
+
 def _routing_of(scoring: str, bias: Tensor | None, num_groups: int, top_groups: int, group_top: int, renormalize: bool,
                 scale: float) -> Routing | None:
     """The registered operator's routing.  No scoring and no setting: softmax and top-k alone (``route_top_k``)."""
@@ -349,6 +359,7 @@ def nvfp4_moe(x: Tensor, router_logits: Tensor, top_k: int, w_gate_up: GroupedNv
     inter = w_gate_up.n // 2
     if w_gate_up.k != h or w_down.k != inter or w_down.n != h or w_down.experts != e:
         raise ValueError("expert weight shapes do not match the activations")
+    _check_logits(router_logits, x, e)
     if routing is not None:
         _check_routing(router_logits, top_k, routing.scoring, routing.bias, routing.num_groups, routing.top_groups,
                        routing.group_top)
