@@ -13,7 +13,9 @@ import torch
 from torch import Tensor
 from torch import is_grad_enabled as _is_grad_enabled
 from torch._C import _are_functorch_transforms_active as _in_transform
+from torch._C import _functorch
 from torch._C import _is_tracing
+from torch.autograd import forward_ad as _forward_ad
 from torch.compiler import is_compiling as _is_compiling
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
@@ -180,6 +182,15 @@ def _direct(*tensors: Tensor | None) -> bool:
     return True
 
 
+def _refuse_tangents(name: str, *tensors: Tensor | None) -> None:
+    """Inside a forward-mode level: an operator without a derivative would drop its inputs' tangents without a word."""
+    for t in tensors:
+        while t is not None and _functorch.is_batchedtensor(t):
+            t = _functorch.get_unwrapped(t)
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"helion_b200::{name} has no forward-mode derivative")
+
+
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation: str | None = None,
            residual: Tensor | None = None, out_dtype: torch.dtype | None = None) -> Tensor:
     """``activation(x @ weight.T + bias) + residual`` in one kernel, rounded once (``torch.ops.helion_b200.linear``).
@@ -196,10 +207,13 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation:
 
     ``K`` must be a multiple of 8.  Operands whose rows are not 16-byte aligned or have no unit stride along K are
     copied first.  Runs on the current stream of ``x``'s device; needs no workspace, so calls on several streams and
-    captured graphs are independent of each other.  Infinities and NaN spread as in the formula.
+    captured graphs are independent of each other.  Infinities and NaN spread as in the formula.  Gradients are refused:
+    in ``backward``, and forward-mode ones in the call.
     """
     activation = activation or "none"
     out_dtype = out_dtype or x.dtype
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("linear", x, weight, bias, residual)
     if _direct(x, weight, bias, residual):
         return _linear_cuda(x, weight, bias, residual, activation, out_dtype)
     _check(x, weight, bias, residual, activation, out_dtype)

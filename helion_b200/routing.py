@@ -14,6 +14,8 @@ from .fused_linear import _cuda_getCurrentRawStream
 from .fused_linear import _cuda_getDevice
 from .fused_linear import _direct
 from .fused_linear import _empty
+from .fused_linear import _forward_ad
+from .fused_linear import _refuse_tangents
 from .ops import _require_cuda
 
 _SCORINGS = {"softmax": 0, "sigmoid": 1}
@@ -133,6 +135,8 @@ def route_experts(router_logits: Tensor, top_k: int, *, scoring: str = "softmax"
     logit of ``+inf``) gets NaN weights and distinct experts.  ``E <= 1024``, ``top_k <= 32``, ``num_groups <= 32``.
     """
     args = (router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("moe_route_experts", router_logits, bias)
     if _direct(router_logits, bias):
         return _route_cuda(*args)
     _check(*args[:7])

@@ -37,3 +37,28 @@ def test_a_trace_records_the_operators(shape):
     assert "helion_b200::moe_route_experts" in str(route.graph)
     logits = torch.randn(7, 8)
     assert all(torch.equal(a, b) for a, b in zip(route(logits), hb.route_experts(logits, 2)))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Neither operator has one; without a word the tangent would be lost."""
+    w, x = torch.randn(8, 16).to(torch.bfloat16), torch.randn(3, 16).to(torch.bfloat16)
+    logits = torch.randn(4, 8)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: hb.linear(dual, w), lambda: hb.linear(x, w, residual=dual[:, :8]),
+                     lambda: hb.route_experts(torch.autograd.forward_ad.make_dual(logits, logits), 2)):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+        assert hb.linear(x, w).shape == (3, 8)  # nothing to lose
+    for transform in (lambda f: torch.func.jvp(f, (x,), (x,)), lambda f: torch.func.jacfwd(f)(x),
+                      lambda f: torch.func.jvp(lambda v: torch.vmap(f)(v), (x,), (x,))):
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            transform(lambda v: hb.linear(v, w))
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda v: hb.route_experts(v, 2)[0], (logits,), (logits,))
+    # without a tangent of their own they run, in any nesting
+    assert torch.func.vmap(lambda v: hb.linear(v, w))(x).shape == (3, 8)
+    inner = torch.func.jvp(lambda v: v + torch.vmap(lambda u: hb.linear(u, w))(x), (x[:, :8],), (x[:, :8],))
+    assert torch.equal(inner[1], x[:, :8])
+    outer = torch.vmap(lambda u: torch.func.jvp(lambda v: v + hb.linear(u, w), (u[:8],), (u[:8],))[1])(x)
+    assert torch.equal(outer, x[:, :8])
