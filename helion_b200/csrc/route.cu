@@ -137,8 +137,8 @@ __device__ __forceinline__ double exact_choice(const Args& a, float logit, int e
   return a.bias != nullptr ? c + double(a.bias[e]) : c;
 }
 
-// Whether the group of this lane stays.  `sure`: its approximate score lies clear above the undecided ones; `near`: it
-// is one of these, and is compared by its exact score.
+// Whether the group of this lane stays.  `sure`: its score lies clear above every group that would go; `near`: it does
+// not, nor clear below every group that would stay, and is compared by its exact score.
 template <typename T>
 __device__ __noinline__ bool refine_groups(const Args& a, const T* row, float top, int group, bool sure, bool near) {
   const int lane = threadIdx.x & 31, lanes = 1 << a.lanes_log;
@@ -321,6 +321,15 @@ __device__ __forceinline__ float choice_error(const Args& a) {
   return a.bias == nullptr ? 0.f : (a.sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18));
 }
 
+// What a group's score s may be off by: `error` for its one or two choices, the rounding of each of these (m1 and, where
+// m2 is above -infinity, m2: a sum can be far smaller than they are; 0 where none was rounded) and of their sum, and what
+// the group's place takes of the key.
+__device__ __forceinline__ float group_error(float s, float m1, float m2, float error, uint32_t group_low) {
+  const float larger = fmaxf(fabsf(m1), m2 > -INFINITY ? fabsf(m2) : 0.f);
+  const float off = error + larger * (1.f / (1 << 23)) + fabsf(s) * (float(group_low + 2) * (1.f / (1 << 23))) + 1e-36f;
+  return fabsf(s) < INFINITY ? off : 0.f;
+}
+
 // How groups lie in the lanes: none, whole lanes (a power of two of them) per group, or anyhow.
 enum Groups { kNoGroups = 0, kLaneGroups = 1, kAnyGroups = 2 };
 
@@ -438,14 +447,14 @@ __device__ __forceinline__ void route_token(const Args& a, int64_t token, const 
     for (int g = 0; g < a.num_groups; ++g) before += __shfl_sync(kAll, s_key, g << a.lanes_log) > s_key;
     bool stays = is_group && before < a.top_groups;
     if (a.top_groups < a.num_groups) {
-      const float last = redux_min(stays ? s : INFINITY), first = redux_max_nan(is_group && !stays ? s : -INFINITY);
-      // sums of two are off by twice as much, scores of logits by a softmax's margin at most, and the key's last bits
-      // are (group_low + 1) 2^-23 of a score; 16-bit logits lose nothing to them
+      // 16-bit logits lose nothing to the key's last bits
       const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
-      const bool exact = error == 0.f && sizeof(T) == 2;
-      const float slack = 2.f * error + fabsf(last) * (float(a.group_low + 3) * (1.f / (1 << 22))) + 1e-36f;
-      if (!exact && first > -INFINITY && last - first <= slack && !spoilt)
-        stays = refine_groups<T>(a, row, top, group, is_group && s > last + slack, is_group && s >= first - slack && s <= last + slack);
+      const float off = group_error(s, biased ? m1 : 0.f, biased && by_scores ? m2 : 0.f, error, a.group_low);
+      const float last = redux_min(stays ? s - off : INFINITY), next = redux_max_nan(is_group && !stays ? s + off : -INFINITY);
+      if (!(error == 0.f && sizeof(T) == 2) && next > -INFINITY && last <= next && !spoilt) {
+        const bool sure = stays && s - off > next;
+        stays = refine_groups<T>(a, row, top, group, sure, is_group && !sure && s + off >= last);
+      }
     }
     if constexpr (GROUPS == kLaneGroups) {
       alive = alive && stays;
@@ -734,11 +743,10 @@ route_many_kernel(const __grid_constant__ Args a) {
         if (g < a.num_groups) before += __shfl_sync(kAll, s_key, (lane & 24) + (g << a.many_lanes_log)) > s_key;
       const bool stays = is_group && before < a.top_groups;
       if (a.top_groups < a.num_groups) {
-        const float last = eight_min(stays ? s : INFINITY), next = eight_max_nan(is_group && !stays ? s : -INFINITY);
-        // (as in route_token, with three bits of a score's key taken by the group)
         const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
-        const float slack = 2.f * error + fabsf(last) * (10.f / (1 << 22)) + 1e-36f;
-        unsure |= !(error == 0.f && sizeof(T) == 2) && next > -INFINITY && last - next <= slack;
+        const float off = group_error(s, biased ? m1 : 0.f, biased && by_scores ? m2 : 0.f, error, 7);
+        const float last = eight_min(stays ? s - off : INFINITY), next = eight_max_nan(is_group && !stays ? s + off : -INFINITY);
+        unsure |= !(error == 0.f && sizeof(T) == 2) && next > -INFINITY && last <= next;
       }
       alive = alive && stays;
     }

@@ -163,3 +163,16 @@ def test_group_scores_beyond_fp32(experts, groups, tokens):
             bias[[0, *range(3, groups)]] = -3.2e38
         for top_k in (2, size):
             check(logits, top_k, scoring="sigmoid", bias=bias.flatten(), num_groups=groups, group_top=2)
+
+
+@pytest.mark.parametrize("tokens", [48, 16403])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size,lead", [(8, 100.0), (8, 1e4), (8, 1e8), (5, 1e4), (2, 1e6), (32, 1e4)])
+def test_group_scores_that_cancel(size, lead, scoring, tokens):
+    """Two choices of opposite sign whose sum is what the groups differ by: far less than the choices' own rounding."""
+    groups = 8
+    g = torch.Generator(device=DEV).manual_seed(size)
+    logits = torch.randn(tokens, groups * size, generator=g, device=DEV)
+    bias = torch.full((groups, size), -2 * lead, device=DEV)
+    bias[:, 0], bias[:, -1] = lead, -lead  # each group's best two; their sum is that of two scores
+    check(logits, 2, scoring=scoring, bias=bias.flatten(), num_groups=groups, top_groups=3, group_top=2)
