@@ -446,12 +446,11 @@ __device__ __forceinline__ void route_token(const Args& a, int64_t token, const 
 #pragma unroll 4
     for (int g = 0; g < a.num_groups; ++g) before += __shfl_sync(kAll, s_key, g << a.lanes_log) > s_key;
     bool stays = is_group && before < a.top_groups;
-    if (a.top_groups < a.num_groups) {
-      // 16-bit logits lose nothing to the key's last bits
-      const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
+    const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
+    if (a.top_groups < a.num_groups && !(error == 0.f && sizeof(T) == 2)) {  // (16-bit logits lose nothing to the keys)
       const float off = group_error(s, biased ? m1 : 0.f, biased && by_scores ? m2 : 0.f, error, a.group_low);
       const float last = redux_min(stays ? s - off : INFINITY), next = redux_max_nan(is_group && !stays ? s + off : -INFINITY);
-      if (!(error == 0.f && sizeof(T) == 2) && next > -INFINITY && last <= next && !spoilt) {
+      if (next > -INFINITY && last <= next && !spoilt) {
         const bool sure = stays && s - off > next;
         stays = refine_groups<T>(a, row, top, group, sure, is_group && !sure && s + off >= last);
       }
@@ -742,11 +741,11 @@ route_many_kernel(const __grid_constant__ Args a) {
       for (int g = 0; g < 8; ++g)
         if (g < a.num_groups) before += __shfl_sync(kAll, s_key, (lane & 24) + (g << a.many_lanes_log)) > s_key;
       const bool stays = is_group && before < a.top_groups;
-      if (a.top_groups < a.num_groups) {
-        const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
+      const float error = base + (convert ? 1.f / (1 << 18) : 0.f);
+      if (a.top_groups < a.num_groups && !(error == 0.f && sizeof(T) == 2)) {
         const float off = group_error(s, biased ? m1 : 0.f, biased && by_scores ? m2 : 0.f, error, 7);
         const float last = eight_min(stays ? s - off : INFINITY), next = eight_max_nan(is_group && !stays ? s + off : -INFINITY);
-        unsure |= !(error == 0.f && sizeof(T) == 2) && next > -INFINITY && last <= next;
+        unsure |= next > -INFINITY && last <= next;
       }
       alive = alive && stays;
     }
