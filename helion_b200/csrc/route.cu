@@ -7,14 +7,17 @@
 //   picks:  the top_k best choices of the experts that stay, equal choices by ascending index, masked experts last
 //   weights: the picks' scores (without the bias), divided by their sum if asked for, times scale
 //
-// Which experts come out is decided as in exact arithmetic: the fast form orders approximate choices that are off by
-// less than half of a margin (below), and where two neighbouring picks, or the last group that stays and the first that
-// goes, are closer than that, those picks (refine_picks) or groups (refine_groups) are compared again in 64 bits: about
-// two rows in a thousand, and what a refinement takes is part of every larger call's time.  Rows with a NaN, rows that
-// have fewer live experts than picks and the rare row in which the candidates themselves are unsure are decided in 64
-// bits from the start (choose_exactly).
+// Which experts come out is decided as in 64 bits (what is equal there goes by ascending index): the fast form orders
+// approximate choices that are off by less than half of a margin (below), and where two neighbouring picks, or the last
+// group that stays and the first that goes, are closer than that, those picks (refine_picks) or groups (refine_groups)
+// are compared again in 64 bits: about two rows in a thousand, and what a refinement takes is part of every larger call's
+// time.  Equal inputs need no comparison, unless something else is near the place where the picks end.  Rows with a NaN,
+// rows that have fewer live experts than picks and rows in which the candidates themselves are unsure (a finite mask of
+// -1e9 on all of a lane's experts stretches the keys until everything else is near everything) are decided in 64 bits
+// from the start (choose_exactly), at ten times the cost.
 //
-// Bound by instructions: at 65536 tokens x 256 experts the bytes take 11 us, and what a warp does per token decides.
+// Bound by instructions and their latency: at 65536 tokens x 256 experts the bytes take 11 us, and what a warp does per
+// token decides.
 //  * a lane holds VPL neighbouring experts, loaded with one or two vector loads; the bias stays in registers;
 //  * the k best choices are no smaller than the smallest of the lanes' best ones (where more than k lanes have any):
 //    that range, [lo, hi], is spread over 22 or 23 bits, which loses no more than fp32 does, and the expert's index,
@@ -582,9 +585,17 @@ route_experts_kernel(const __grid_constant__ Args a) {
 // tokens' rows are on their way meanwhile) and keeps its four best keys.  The range of the keys starts at the smallest
 // of the lanes' second-best choices where that leaves enough experts in it.  Tokens with near ties among their picks have
 // these compared in 64 bits afterwards, by the whole warp; a token with anything else unsure goes through route_token.
-// 65536 tokens x 256 experts, top 8: 43 us in groups (top 4 of 8, biased sigmoid) against 61 with a warp per token, 31
-// against 38 by softmax; 128 experts in bf16 21 against 34.  In smaller batches the longer work per warp shows as latency: 8192 tokens in groups
-// 13 against 12 us, by softmax 6.3 against 7.0; hence the bounds in launch_many.
+// 65536 tokens x 256 experts, top 8: 46 us in groups (top 4 of 8, biased sigmoid) against 63 with a warp per token, 32
+// against 39 by softmax; 128 experts in bf16 22 against 35, 64 in fp32 16 against 29.  410 instructions per token, issue
+// slots busy 59 % at 14 warps per SM (128 registers): instructions and their latency share the time.  In smaller batches
+// the longer work per warp shows as latency, hence the bounds in launch_many.  Here / a warp per token, fp32, top 6:
+//   by softmax    4096 tokens   8192        16384       groups        8192        16384       32768
+//   32 experts    3.2 / 2.8     5.1 / 4.1   6.2 / 6.5
+//   64            3.6 / 3.5     4.4 / 5.6   6.6 / 8.4                 7.2 / 7.9   9.2 / 13.1  18.1 / 24.9
+//   96            4.0 / 4.0     5.0 / 6.0   7.6 / 9.1
+//   128           4.0 / 4.0     6.2 / 6.0   9.0 / 9.1                 12.7 / 10.3 16.6 / 14.3 20.9 / 27.8
+//   192           4.6 / 5.0     7.2 / 7.3   10.3 / 10.8               8.8 / 13.6  18.4 / 21.1 25.2 / 37.4
+//   256           4.5 / 4.9     6.2 / 7.3   10.1 / 10.7               13.4 / 12.2 18.8 / 18.1 25.6 / 31.4
 constexpr int kManyWarps = 4;
 constexpr int kManyMaxPicks = 8;
 

@@ -129,10 +129,13 @@ def route_experts(router_logits: Tensor, top_k: int, *, scoring: str = "softmax"
       choices, and only the best ``top_groups`` groups' experts can be picked.
     * weights: the picked experts' scores, divided by their sum with ``renormalize``, times ``scale``.
 
-    The picks are those of exact arithmetic: where two choices are too close for fp32 the row is decided in 64 bits.
+    The picks are those of an evaluation in 64 bits: where two choices are too close for fp32 they are compared in 64, and
+    what is equal there goes by ascending index.
     A logit of ``-inf`` masks an expert: it counts in no sum, is picked only when nothing else is left (ascending
     index) and gets weight 0; a row with every expert masked gets weights 0.  A row with a NaN (or, under softmax, a
-    logit of ``+inf``) gets NaN weights and distinct experts.  ``E <= 1024``, ``top_k <= 32``, ``num_groups <= 32``.
+    logit of ``+inf``) gets NaN weights and distinct experts.  A large finite logit in place of ``-inf`` is a logit like
+    any other: right, but without a bias many such rows are decided in 64 bits throughout (65536 x 256 with the last 32 at
+    -1e9: 440 us, at ``-inf`` 36).  ``E <= 1024``, ``top_k <= 32``, ``num_groups <= 32``.
     """
     args = (router_logits, top_k, scoring, bias, num_groups, top_groups, group_top, renormalize, scale)
     if _forward_ad._current_level >= 0:
